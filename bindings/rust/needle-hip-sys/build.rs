@@ -5,16 +5,19 @@
 //   -ffp-contract=off                          one rounding per multiply and per add in the exact re-scoring kernels
 //   -fhip-fp32-correctly-rounded-divide-sqrt   IEEE sqrt and divide, as the reference's scalar Rust
 //   flat_scan_bf16.hip additionally            -mllvm -amdgpu-mfma-vgpr-form=1 -fno-honor-nans
+//   int8.hip and beam.hip additionally         -Xclang -target-feature -Xclang -packed-fp32-ops
 use std::{env, path::PathBuf, process::Command};
 
 const SOURCES: &[&str] = &[
     "api.hip", "api_ivf.hip", "api_adc.hip", "flat_scan.hip", "flat_scan_bf16.hip", "flat_post.hip", "prep.hip", "adc.hip",
-    "binary.hip", "train.hip", "adaptive.hip", "ops.hip", "comm.hip",
+    "binary.hip", "train.hip", "adaptive.hip", "ops.hip", "comm.hip", "int8.hip", "beam.hip",
 ];
 const FLAGS: &[&str] = &[
     "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-ffp-contract=off", "-fhip-fp32-correctly-rounded-divide-sqrt",
     "-Wall", "-Wno-unused-function",
 ];
+const OPERATOR_SOURCES: &[&str] = &["int8.hip", "beam.hip"];
+const OPERATOR_FLAGS: &[&str] = &["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"];
 const BF16_SCAN_FLAGS: &[&str] = &["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-fno-honor-nans"];
 
 fn main() {
@@ -42,6 +45,9 @@ fn main() {
         cmd.args(FLAGS);
         if *f == "flat_scan_bf16.hip" {
             cmd.args(BF16_SCAN_FLAGS);
+        }
+        if OPERATOR_SOURCES.contains(f) {
+            cmd.args(OPERATOR_FLAGS);
         }
         let st = cmd.arg("-c").arg(src.join(f)).arg("-o").arg(&o).status().expect("hipcc not found");
         assert!(st.success(), "hipcc failed on {f}");

@@ -56,7 +56,42 @@ pub const NEEDLE_PRECISION_EXACT_SCAN: i32 = 2;
 
 pub const NEEDLE_HALF_F16: c_int = 0;
 pub const NEEDLE_HALF_BF16: c_int = 1;
+pub const NEEDLE_VALUE_F32: c_int = 0;
+pub const NEEDLE_VALUE_F16: c_int = 1;
+pub const NEEDLE_VALUE_BF16: c_int = 2;
 pub const NEEDLE_HIP_UNIQUE_ID_BYTES: usize = 128;
+
+#[repr(C)]
+pub struct needle_beam_params {
+    pub groups: u32,
+    pub beams: u32,
+    pub vocab: u32,
+    pub k: u32,
+    pub value: i32,
+    pub normalize: i32,
+    pub row_stride: u64,
+    pub scores: *const f32,
+    pub finished: *const u8,
+    pub mask: *const u32,
+    pub mask_stride: u64,
+    pub end_token: u32,
+    pub reserved: u32,
+}
+
+#[repr(C)]
+pub struct needle_beam_state {
+    pub src: *const c_void,
+    pub dst: *mut c_void,
+    pub outer: u64,
+    pub inner: u64,
+    pub bytes: u64,
+    pub src_outer_stride: u64,
+    pub src_row_stride: u64,
+    pub src_inner_stride: u64,
+    pub dst_outer_stride: u64,
+    pub dst_row_stride: u64,
+    pub dst_inner_stride: u64,
+}
 
 #[repr(C)]
 pub struct needle_search_params {
@@ -143,6 +178,14 @@ extern "C" {
     pub fn needle_hip_distance_matrix_device(ctx: *mut needle_hip_ctx, metric: c_int, arith: c_int, d_queries: *const f32, q: u32, d_base: *const f32, n: u64, dim: u32, d_out: *mut f32) -> c_int;
     pub fn needle_hip_multi_query_search(ctx: *mut needle_hip_ctx, metric: c_int, arith: c_int, queries: *const f32, q: u32, base: *const f32, n: u64, dim: u32, k: u32, out_idx: *mut u64, out_dists: *mut f32, out_counts: *mut u32) -> c_int;
     pub fn needle_hip_multi_query_search_device(ctx: *mut needle_hip_ctx, metric: c_int, arith: c_int, d_queries: *const f32, q: u32, d_base: *const f32, n: u64, dim: u32, k: u32, d_out_idx: *mut u64, d_out_dists: *mut f32, d_out_counts: *mut u32) -> c_int;
+    pub fn needle_hip_quantize_rows_i8(ctx: *mut needle_hip_ctx, rows: *const c_void, value: c_int, n: u64, dim: u32, out_codes: *mut i8, out_scales: *mut f32) -> c_int;
+    pub fn needle_hip_quantize_rows_i8_device(ctx: *mut needle_hip_ctx, d_rows: *const c_void, value: c_int, n: u64, dim: u32, row_stride: u64, d_out_codes: *mut i8, code_stride: u64, d_out_scales: *mut f32) -> c_int;
+    pub fn needle_hip_matmul_i8(ctx: *mut needle_hip_ctx, a: *const i8, a_scales: *const f32, m: u32, b: *const i8, b_scales: *const f32, n: u64, k: u32, bias: *const f32, out: *mut f32) -> c_int;
+    pub fn needle_hip_matmul_i8_device(ctx: *mut needle_hip_ctx, d_a: *const i8, a_stride: u64, d_a_scales: *const f32, m: u32, d_b: *const i8, b_stride: u64, d_b_scales: *const f32, n: u64, k: u32, d_bias: *const f32, out_value: c_int, d_out: *mut c_void, out_stride: u64) -> c_int;
+    pub fn needle_hip_linear_i8_device(ctx: *mut needle_hip_ctx, d_x: *const c_void, x_value: c_int, x_stride: u64, m: u32, d_b: *const i8, b_stride: u64, d_b_scales: *const f32, n: u64, k: u32, d_bias: *const f32, out_value: c_int, d_out: *mut c_void, out_stride: u64) -> c_int;
+    pub fn needle_hip_beam_select(ctx: *mut needle_hip_ctx, params: *const needle_beam_params, logits: *const c_void, out_parents: *mut u32, out_tokens: *mut u32, out_scores: *mut f32, out_counts: *mut u32) -> c_int;
+    pub fn needle_hip_beam_select_device(ctx: *mut needle_hip_ctx, params: *const needle_beam_params, d_logits: *const c_void, states: *const needle_beam_state, n_states: u32, d_out_parents: *mut u32, d_out_tokens: *mut u32, d_out_scores: *mut f32, d_out_counts: *mut u32) -> c_int;
+    pub fn needle_hip_beam_reorder_device(ctx: *mut needle_hip_ctx, d_parents: *const u32, groups: u32, beams: u32, k: u32, states: *const needle_beam_state, n_states: u32) -> c_int;
     pub fn needle_hip_comm_unique_id(out_id: *mut u8) -> c_int;
     pub fn needle_hip_comm_init(ctx: *mut needle_hip_ctx, unique_id: *const u8, rank: c_int, world: c_int, out: *mut *mut needle_hip_comm) -> c_int;
     pub fn needle_hip_comm_destroy(comm: *mut needle_hip_comm);

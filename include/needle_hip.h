@@ -507,6 +507,112 @@ needle_hip_status needle_hip_multi_query_search_device(needle_hip_ctx* ctx, need
                                                        uint64_t n, uint32_t dim, uint32_t k, uint64_t* d_out_idx,
                                                        float* d_out_dists, uint32_t* d_out_counts);
 
+/* ---- rows in 8-bit integers, their products, and the best continuations --------
+ * Operators next to distance_matrix and batch_top_k for the models whose embeddings
+ * an index holds; they have no counterpart in the reference.  Like every call here
+ * they work on the context's stream and return when the work is done (so they cannot
+ * be recorded under stream capture), take the context's lock, and may be called from
+ * several threads.  Strides are in ELEMENTS of the array they belong to unless they
+ * say bytes; no alignment beyond the element's own is required.  An output must not
+ * overlap an input or another output. */
+
+/* Type of the values of an array in floating point. */
+typedef enum needle_value { NEEDLE_VALUE_F32 = 0, NEEDLE_VALUE_F16 = 1, NEEDLE_VALUE_BF16 = 2 } needle_value;
+
+/* Rows to int8 with one scale each, symmetric around zero:
+ *     scale[i] = max_j |x[i][j]| * (1 / 127)           (in f32, by the f32 nearest to 1 / 127)
+ *     code[i][j] = the whole number nearest to x[i][j] / scale[i], ties to even
+ * The quotient is the exact one of the two f32 numbers, clamped to -127 .. 127.  A row
+ * of zeros (or whose scale underflows to 0) has scale 0 and codes 0; a row that holds a
+ * NaN or an infinity has scale NaN and codes 0, which makes its products NaN.  value:
+ * needle_value of the rows; codes: n rows of code_stride >= dim; dim 0 gives scale 0.
+ * The host form takes and gives contiguous rows and refuses NaN / Inf with
+ * NEEDLE_HIP_ERR_INVALID_VECTOR. */
+needle_hip_status needle_hip_quantize_rows_i8(needle_hip_ctx* ctx, const void* rows, int value, uint64_t n, uint32_t dim,
+                                              int8_t* out_codes, float* out_scales);
+needle_hip_status needle_hip_quantize_rows_i8_device(needle_hip_ctx* ctx, const void* d_rows, int value, uint64_t n,
+                                                     uint32_t dim, uint64_t row_stride, int8_t* d_out_codes,
+                                                     uint64_t code_stride, float* d_out_scales);
+
+/* out[i][j] = (sum_x a[i][x] * b[j][x]) * a_scales[i] * b_scales[j] (+ bias[j]): m rows
+ * of codes against n, each with its scale (a: queries or tokens, b: base rows or the
+ * output channels of a layer).  The sum is exact in 32-bit integers, which k <= 131071
+ * guarantees for any codes (-128 included); it is turned into f32, multiplied by the
+ * two scales in that order, the bias (nullable) is added, and the result is rounded once
+ * more where out_value (needle_value) is a half type.  k may be a prefix of longer rows (stride
+ * above k).  m * n may be any size, n < 2^31.  k 0 gives the bias, or zeros. */
+needle_hip_status needle_hip_matmul_i8(needle_hip_ctx* ctx, const int8_t* a, const float* a_scales, uint32_t m,
+                                       const int8_t* b, const float* b_scales, uint64_t n, uint32_t k,
+                                       const float* bias, float* out);
+needle_hip_status needle_hip_matmul_i8_device(needle_hip_ctx* ctx, const int8_t* d_a, uint64_t a_stride,
+                                              const float* d_a_scales, uint32_t m, const int8_t* d_b, uint64_t b_stride,
+                                              const float* d_b_scales, uint64_t n, uint32_t k, const float* d_bias,
+                                              int out_value, void* d_out, uint64_t out_stride);
+
+/* The same product for rows that are still in floating point (x_value): they are
+ * quantized as needle_hip_quantize_rows_i8_device does, into the context's workspace, and
+ * multiplied; results equal the two calls made one after the other. */
+needle_hip_status needle_hip_linear_i8_device(needle_hip_ctx* ctx, const void* d_x, int x_value, uint64_t x_stride,
+                                              uint32_t m, const int8_t* d_b, uint64_t b_stride, const float* d_b_scales,
+                                              uint64_t n, uint32_t k, const float* d_bias, int out_value, void* d_out,
+                                              uint64_t out_stride);
+
+/* One step of a beam search.  `groups` requests keep `beams` beams each; row g * beams + b
+ * of the logits holds beam b's score for each of `vocab` continuations (tokens of a
+ * vocabulary, or base rows of a retrieval hop).  A continuation's total is
+ *     normalize 0: scores[row] + x        normalize 1: scores[row] + (x - log sum exp x)
+ * with the sum over the row's admitted continuations.  The k best of a group by (total
+ * descending, beam, token) are its picks; continuations of one beam rank by their logits.
+ * Totals are formed and compared in 64 bits and reported rounded to f32.  Not offered: what the mask leaves out, totals of -inf or
+ * NaN (so a beam whose score is -inf or NaN offers nothing; nor does, under normalize, a
+ * row with an admitted NaN or +inf).  An ended beam offers one continuation: end_token
+ * with scores[row] as its total; its row of logits and its mask are not looked at.
+ * k <= 256, beams <= 1024, beams * vocab < 2^32, groups * beams < 2^31. */
+typedef struct needle_beam_params {
+    uint32_t groups, beams, vocab, k;
+    int32_t value;            /* needle_value of the logits */
+    int32_t normalize;
+    uint64_t row_stride;      /* elements between rows of the logits, >= vocab */
+    const float* scores;      /* [groups * beams] running scores; NULL = zeros */
+    const uint8_t* finished;  /* [groups * beams] non-zero = an ended beam; NULL = none */
+    const uint32_t* mask;     /* admitted continuations, bit t & 31 of word t >> 5 of a row; NULL = all */
+    uint64_t mask_stride;     /* words between the rows' masks (0 = one mask for all rows) */
+    uint32_t end_token;
+    uint32_t reserved;        /* 0 */
+} needle_beam_params;
+
+/* Something every beam carries (keys and values, a query vector, a history): after the
+ * picks, row g * k + j of dst becomes a copy of row g * beams + parent of src.  A row is
+ * outer x inner runs of `bytes` bytes; all strides are in bytes.  Rows of places without
+ * a pick stay as they were.  dst must not overlap any src or another dst. */
+typedef struct needle_beam_state {
+    const void* src;
+    void* dst;
+    uint64_t outer, inner, bytes;
+    uint64_t src_outer_stride, src_row_stride, src_inner_stride;
+    uint64_t dst_outer_stride, dst_row_stride, dst_inner_stride;
+} needle_beam_state;
+
+/* Picks of every group, best first: [groups][k] beam within the group, continuation and
+ * total; counts[g] of them, the rest of a row is padded with UINT32_MAX / UINT32_MAX /
+ * -inf.  k <= 256, at most 256 states.  The pointers in params are host pointers in the host form (contiguous logits:
+ * row_stride is ignored, and mask_stride is 0 or ceil(vocab / 32)), device pointers in
+ * the device form; params and the array of states itself lie on the host.  states may be
+ * NULL when n_states is 0. */
+needle_hip_status needle_hip_beam_select(needle_hip_ctx* ctx, const needle_beam_params* params, const void* logits,
+                                         uint32_t* out_parents, uint32_t* out_tokens, float* out_scores,
+                                         uint32_t* out_counts);
+needle_hip_status needle_hip_beam_select_device(needle_hip_ctx* ctx, const needle_beam_params* params, const void* d_logits,
+                                                const needle_beam_state* states, uint32_t n_states,
+                                                uint32_t* d_out_parents, uint32_t* d_out_tokens, float* d_out_scores,
+                                                uint32_t* d_out_counts);
+
+/* The move of the states alone, for picks made elsewhere: parents [groups][k] on the
+ * device; an entry of `beams` or more (UINT32_MAX among them) leaves its row as it was. */
+needle_hip_status needle_hip_beam_reorder_device(needle_hip_ctx* ctx, const uint32_t* d_parents, uint32_t groups,
+                                                 uint32_t beams, uint32_t k, const needle_beam_state* states,
+                                                 uint32_t n_states);
+
 /* ---- row-sharded search over the GPUs of one node --------------------------- */
 
 /* MultiGpuShardManager, src/experimental/gpu/mod.rs:1269-1383, as one process per

@@ -18,6 +18,8 @@ OK, ERR_DIMENSION_MISMATCH, ERR_INVALID_VECTOR, ERR_INVALID_ARGUMENT, ERR_OUT_OF
 
 # needle_precision
 PRECISION_FP32, PRECISION_BF16, PRECISION_EXACT_SCAN = range(3)
+# needle_value
+VALUE_F32, VALUE_F16, VALUE_BF16 = range(3)
 # needle_arith
 ARITH_DISTANCE_RS, ARITH_ACCEL_CHUNK4, ARITH_SERVICE, ARITH_AVX2, ARITH_AVX512, ARITH_NEON = range(6)
 
@@ -39,6 +41,8 @@ EXPORTS = (
     "needle_hip_merge_shard_slots_device",
     "needle_hip_distance_matrix", "needle_hip_distance_matrix_device", "needle_hip_multi_query_search",
     "needle_hip_multi_query_search_device",
+    "needle_hip_quantize_rows_i8", "needle_hip_quantize_rows_i8_device", "needle_hip_matmul_i8", "needle_hip_matmul_i8_device",
+    "needle_hip_linear_i8_device", "needle_hip_beam_select", "needle_hip_beam_select_device", "needle_hip_beam_reorder_device",
 )
 
 UNIQUE_ID_BYTES = 128
@@ -47,6 +51,18 @@ UNIQUE_ID_BYTES = 128
 class SearchParams(C.Structure):
     _fields_ = [("k", C.c_uint32), ("nprobe", C.c_uint32), ("precision", C.c_int32), ("reserved", C.c_uint32),
                 ("filter_bitmask", C.c_void_p)]
+
+
+class BeamParams(C.Structure):
+    _fields_ = [("groups", C.c_uint32), ("beams", C.c_uint32), ("vocab", C.c_uint32), ("k", C.c_uint32), ("value", C.c_int32),
+                ("normalize", C.c_int32), ("row_stride", C.c_uint64), ("scores", C.c_void_p), ("finished", C.c_void_p),
+                ("mask", C.c_void_p), ("mask_stride", C.c_uint64), ("end_token", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class BeamState(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("outer", C.c_uint64), ("inner", C.c_uint64), ("bytes", C.c_uint64),
+                ("src_outer_stride", C.c_uint64), ("src_row_stride", C.c_uint64), ("src_inner_stride", C.c_uint64),
+                ("dst_outer_stride", C.c_uint64), ("dst_row_stride", C.c_uint64), ("dst_inner_stride", C.c_uint64)]
 
 
 class Metrics(C.Structure):
@@ -199,6 +215,22 @@ def lib() -> C.CDLL:
         getattr(L, name).argtypes = [vp, i32, i32, vp, u32, vp, u64, u32, u32, vp, vp, vp]
     L.needle_hip_batch_top_k_device_noalloc.restype = i32
     L.needle_hip_batch_top_k_device_noalloc.argtypes = [vp, vp, u32, u64, u32, vp, vp, vp]
+    L.needle_hip_quantize_rows_i8.restype = i32
+    L.needle_hip_quantize_rows_i8.argtypes = [vp, vp, i32, u64, u32, vp, vp]
+    L.needle_hip_quantize_rows_i8_device.restype = i32
+    L.needle_hip_quantize_rows_i8_device.argtypes = [vp, vp, i32, u64, u32, u64, vp, u64, vp]
+    L.needle_hip_matmul_i8.restype = i32
+    L.needle_hip_matmul_i8.argtypes = [vp, vp, vp, u32, vp, vp, u64, u32, vp, vp]
+    L.needle_hip_matmul_i8_device.restype = i32
+    L.needle_hip_matmul_i8_device.argtypes = [vp, vp, u64, vp, u32, vp, u64, vp, u64, u32, vp, i32, vp, u64]
+    L.needle_hip_linear_i8_device.restype = i32
+    L.needle_hip_linear_i8_device.argtypes = [vp, vp, i32, u64, u32, vp, u64, vp, u64, u32, vp, i32, vp, u64]
+    L.needle_hip_beam_select.restype = i32
+    L.needle_hip_beam_select.argtypes = [vp, C.POINTER(BeamParams), vp, vp, vp, vp, vp]
+    L.needle_hip_beam_select_device.restype = i32
+    L.needle_hip_beam_select_device.argtypes = [vp, C.POINTER(BeamParams), vp, C.POINTER(BeamState), u32, vp, vp, vp, vp]
+    L.needle_hip_beam_reorder_device.restype = i32
+    L.needle_hip_beam_reorder_device.argtypes = [vp, vp, u32, u32, u32, C.POINTER(BeamState), u32]
     L.needle_hip_comm_unique_id.restype = i32
     L.needle_hip_comm_unique_id.argtypes = [vp]
     L.needle_hip_comm_init.restype = i32

@@ -1,0 +1,76 @@
+// Arrays in floating point that an operator takes or gives in one of three types (needle_value), and what the host side
+// of such operators checks.
+#pragma once
+#include "nh_api.h"
+
+namespace nh {
+
+__host__ __device__ inline uint32_t value_size(int value) { return value == NEEDLE_VALUE_F32 ? 4u : 2u; }
+inline bool value_known(int value) {
+    return value == NEEDLE_VALUE_F32 || value == NEEDLE_VALUE_F16 || value == NEEDLE_VALUE_BF16;
+}
+
+// A loaded pattern widened to f32 (exact), and an f32 rounded to the type (nearest, ties to even).
+struct ValueF32 {
+    typedef uint32_t bits;
+    static constexpr int size = 4;
+    __device__ static float widen(uint32_t u) { return __uint_as_float(u); }
+    __device__ static uint32_t round(float f) { return __float_as_uint(f); }
+};
+struct ValueF16 {
+    typedef uint16_t bits;
+    static constexpr int size = 2;
+    __device__ static float widen(uint16_t u) { return (float)__builtin_bit_cast(_Float16, u); }
+    __device__ static uint16_t round(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
+};
+struct ValueBF16 {
+    typedef uint16_t bits;
+    static constexpr int size = 2;
+    __device__ static float widen(uint16_t u) { return __uint_as_float((uint32_t)u << 16); }
+    __device__ static uint16_t round(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
+};
+
+// 16 bytes at any address the element type allows: the target's global loads and stores need no more alignment than that.
+struct __attribute__((packed, aligned(1))) bytes16_t { uint32_t w[4]; };
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+
+// Makes `device` current for one call and gives the caller's own back on return.
+class DeviceScope {
+public:
+    explicit DeviceScope(int device) {
+        e_ = hipGetDevice(&was_);
+        if (e_ == hipSuccess && was_ != device) {
+            e_ = hipSetDevice(device);
+            moved_ = e_ == hipSuccess;
+        }
+    }
+    ~DeviceScope() {
+        if (moved_) (void)hipSetDevice(was_);
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+    hipError_t error() const { return e_; }
+private:
+    int was_ = 0;
+    bool moved_ = false;
+    hipError_t e_ = hipSuccess;
+};
+
+// Bytes from the first to behind the last element of `rows` rows of `len` elements, `stride` apart; false on overflow.
+inline bool span_bytes(uint64_t rows, uint64_t len, uint64_t stride, uint64_t size, uint64_t* out) {
+    *out = 0;
+    if (rows == 0 || len == 0) return true;
+    uint64_t last, all;
+    if (__builtin_mul_overflow(rows - 1, stride, &last) || __builtin_add_overflow(last, len, &all) ||
+        __builtin_mul_overflow(all, size, &all) || all > (1ull << 62))
+        return false;
+    *out = all;
+    return true;
+}
+inline bool ranges_meet(const void* a, uint64_t na, const void* b, uint64_t nb) {
+    const uint64_t x = (uint64_t)a, y = (uint64_t)b;
+    return a && b && na && nb && x < y + nb && y < x + na;
+}
+
+}  // namespace nh

@@ -53,6 +53,51 @@ def _wait_for_producer(t) -> None:
         torch.cuda.current_stream(t.device).synchronize()
 
 
+_VALUES = {"torch.float32": _lib.VALUE_F32, "torch.float16": _lib.VALUE_F16, "torch.bfloat16": _lib.VALUE_BF16}
+
+
+def _value(t, what: str) -> int:
+    v = _VALUES.get(str(t.dtype))
+    if v is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
+    return v
+
+
+def _codes_i8(codes, scales, what: str):
+    """Host int8 codes [rows, dim] and their f32 scales, contiguous.  Values are not converted: a wider type would wrap."""
+    c, s = np.ascontiguousarray(codes), _f32(scales).reshape(-1)
+    if c.dtype != np.int8 or c.ndim != 2 or s.size != c.shape[0]:
+        raise ValueError(f"{what} must be int8 [rows, dim] with one scale per row")
+    return c, s
+
+
+def _state_layout(src, dst, axis: int):
+    """(outer, inner, bytes, strides of src, strides of dst) in bytes of two tensors whose dimension `axis` numbers the
+    rows: dimensions before it must fold into one, those behind it into runs of neighbouring elements that lie one stride
+    apart."""
+    def fold(dims):  # [(size, src stride, dst stride)]: neighbours that continue each other in both tensors become one
+        out = []
+        for n, a, b in dims:
+            if n == 1:
+                continue
+            if out and out[-1][1] == n * a and out[-1][2] == n * b:
+                out[-1] = (out[-1][0] * n, a, b)
+            else:
+                out.append((n, a, b))
+        return out
+
+    size = src.element_size()
+    dims = [(int(n), int(a) * size, int(b) * size) for n, a, b in zip(src.shape, src.stride(), dst.stride())]
+    before, behind = fold(dims[:axis]), fold(dims[axis + 1:])
+    run = size
+    if behind and behind[-1][1] == behind[-1][2] == size:
+        run *= behind.pop()[0]
+    if len(before) > 1 or len(behind) > 1:
+        raise ValueError("a state's dimensions must fold into one before its rows and, behind them, into runs one stride apart")
+    outer, inner = before[0] if before else (1, 0, 0), behind[0] if behind else (1, 0, 0)
+    return outer[0], inner[0], run, (outer[1], int(src.stride(axis)) * size, inner[1]), (outer[2], int(dst.stride(axis)) * size, inner[2])
+
+
 def _destroy_handle(owner, destroy_name: str = "needle_hip_index_destroy") -> None:
     """Destroys owner._h unless the context it is bound to has been closed: closing a context frees everything bound to
     it, and a wrapper that outlives its context (garbage collected later) must not hand the dead handle to the library
@@ -219,6 +264,206 @@ class Context:
         _lib.check(_lib.lib().needle_hip_merge_topk_device(self._h, d_dists.data_ptr(), d_ids.data_ptr(),
                                                            d_counts.data_ptr(), lists, q, per, k, d_out_ids.data_ptr(),
                                                            d_out_dists.data_ptr(), d_out_counts.data_ptr()))
+
+    # ---- rows in 8-bit integers, their products, the best continuations ---------------------------------------------
+    def _check_device(self, **tensors) -> None:
+        """Every given tensor lies on the context's device; the caller's stream there has finished."""
+        for name, t in tensors.items():
+            if t is not None and (not getattr(t, "is_cuda", False) or t.device.index != self.device):
+                raise ValueError(f"{name} must be a tensor on device {self.device}")
+        _wait_for_producer(next(t for t in tensors.values() if t is not None))
+
+    @staticmethod
+    def _check_rows(t, name: str, dtype=None, cols=None, rows=None) -> None:
+        """A matrix whose rows are contiguous (any stride between them)."""
+        if t.dim() != 2 or (dtype is not None and str(t.dtype) != dtype) or (cols is not None and int(t.shape[1]) != cols) or \
+                (rows is not None and int(t.shape[0]) != rows):
+            raise ValueError(f"{name} must be [{'n' if rows is None else rows}, {'dim' if cols is None else cols}]"
+                             f"{'' if dtype is None else ' of ' + dtype}, not {list(t.shape)} of {t.dtype}")
+        if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            raise ValueError(f"{name} must have contiguous rows that do not overlap")
+
+    @staticmethod
+    def _check_flat(t, name: str, dtype: str, size: int) -> None:
+        if str(t.dtype) != dtype or int(t.numel()) != size or not t.is_contiguous():
+            raise ValueError(f"{name} must be {size} contiguous values of {dtype}, not {list(t.shape)} of {t.dtype}")
+
+    @staticmethod
+    def _stride(t) -> int:
+        return int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1])
+
+    def quantize_rows(self, rows):
+        """(codes int8 [n, dim], scales f32 [n]) of float32 or float16 host rows: symmetric, scale = max |x| * (1 / 127) per row in f32,
+        codes the whole numbers nearest to x / scale (needle_hip_quantize_rows_i8).  NaN / Inf raise InvalidVector."""
+        r = np.asarray(rows)
+        r = np.ascontiguousarray(r, dtype=np.float16 if r.dtype == np.float16 else np.float32)
+        if r.ndim != 2:
+            raise ValueError("rows must be [n, dim]")
+        codes, scales = np.zeros(r.shape, dtype=np.int8), np.zeros(r.shape[0], dtype=np.float32)
+        _lib.check(_lib.lib().needle_hip_quantize_rows_i8(self._h, r.ctypes.data, _lib.VALUE_F16 if r.dtype == np.float16 else _lib.VALUE_F32,
+                                                          r.shape[0], r.shape[1], codes.ctypes.data, scales.ctypes.data))
+        return codes, scales
+
+    def quantize_rows_device(self, d_rows, d_codes, d_scales) -> None:
+        """The same for a float32 / float16 / bfloat16 device matrix, into int8 [n, dim] codes and float32 [n] scales; rows may
+        lie apart.  A row with a NaN or an infinity gets scale NaN and codes 0."""
+        self._check_rows(d_rows, "d_rows")
+        n, dim = int(d_rows.shape[0]), int(d_rows.shape[1])
+        value = _value(d_rows, "d_rows")
+        self._check_rows(d_codes, "d_codes", "torch.int8", dim, n)
+        self._check_flat(d_scales, "d_scales", "torch.float32", n)
+        self._check_device(d_rows=d_rows, d_codes=d_codes, d_scales=d_scales)
+        _lib.check(_lib.lib().needle_hip_quantize_rows_i8_device(self._h, d_rows.data_ptr(), value, n, dim, self._stride(d_rows),
+                                                                 d_codes.data_ptr(), self._stride(d_codes), d_scales.data_ptr()))
+
+    def matmul_i8(self, a, a_scales, b, b_scales, bias=None) -> np.ndarray:
+        """f32 [m, n] of (a[i] . b[j]) * a_scales[i] * b_scales[j] (+ bias[j]) for int8 host codes [m, k] and [n, k]
+        (needle_hip_matmul_i8)."""
+        a, sa = _codes_i8(a, a_scales, "a")
+        b, sb = _codes_i8(b, b_scales, "b")
+        if a.shape[1] != b.shape[1]:
+            raise _lib.DimensionMismatch(_lib.ERR_DIMENSION_MISMATCH, f"Dimension mismatch: {a.shape[1]} and {b.shape[1]}")
+        t = None if bias is None else _f32(bias).reshape(-1)
+        if t is not None and t.size != b.shape[0]:
+            raise ValueError("bias must have one value per row of b")
+        out = np.empty((a.shape[0], b.shape[0]), dtype=np.float32)
+        _lib.check(_lib.lib().needle_hip_matmul_i8(self._h, a.ctypes.data, sa.ctypes.data, a.shape[0], b.ctypes.data, sb.ctypes.data,
+                                                   b.shape[0], a.shape[1], None if t is None else t.ctypes.data, out.ctypes.data))
+        return out
+
+    def matmul_i8_device(self, d_a, d_a_scales, d_b, d_b_scales, d_out, d_bias=None) -> None:
+        """The same on the device, into a float32 / float16 / bfloat16 [m, n] matrix.  Rows of every matrix may lie apart: the
+        first k codes of longer rows (a Matryoshka prefix) are a view like any other."""
+        self._product(d_a, d_a_scales, d_b, d_b_scales, d_out, d_bias)
+
+    def linear_i8_device(self, d_x, d_b, d_b_scales, d_out, d_bias=None) -> None:
+        """matmul_i8_device for rows that are still in floating point: they are quantized as quantize_rows_device does and
+        multiplied in one call."""
+        self._product(d_x, None, d_b, d_b_scales, d_out, d_bias)
+
+    def _product(self, d_a, d_a_scales, d_b, d_b_scales, d_out, d_bias) -> None:
+        self._check_rows(d_a, "the rows", None if d_a_scales is None else "torch.int8")
+        m, k = int(d_a.shape[0]), int(d_a.shape[1])
+        self._check_rows(d_b, "d_b", "torch.int8")
+        if int(d_b.shape[1]) != k:
+            raise _lib.DimensionMismatch(_lib.ERR_DIMENSION_MISMATCH, f"Dimension mismatch: {k} and {int(d_b.shape[1])}")
+        n = int(d_b.shape[0])
+        self._check_rows(d_out, "d_out", None, n, m)
+        out_value = _value(d_out, "d_out")
+        for t, name, size in ((d_a_scales, "d_a_scales", m), (d_b_scales, "d_b_scales", n), (d_bias, "d_bias", n)):
+            if t is not None:
+                self._check_flat(t, name, "torch.float32", size)
+        x_value = _value(d_a, "d_x") if d_a_scales is None else None
+        self._check_device(a=d_a, a_scales=d_a_scales, d_b=d_b, d_b_scales=d_b_scales, d_out=d_out, d_bias=d_bias)
+        right = (m, d_b.data_ptr(), self._stride(d_b), d_b_scales.data_ptr(), n, k, None if d_bias is None else d_bias.data_ptr(), out_value,
+                 d_out.data_ptr(), self._stride(d_out))
+        if d_a_scales is None:
+            _lib.check(_lib.lib().needle_hip_linear_i8_device(self._h, d_a.data_ptr(), x_value, self._stride(d_a), *right))
+        else:
+            _lib.check(_lib.lib().needle_hip_matmul_i8_device(self._h, d_a.data_ptr(), self._stride(d_a), d_a_scales.data_ptr(), *right))
+
+    def beam_select(self, logits, scores, k: int, *, beams: int, normalize: bool = True, mask=None, finished=None, end_token: int = 0):
+        """(parents, tokens uint32, scores f32, all [groups, k], counts uint32 [groups]): the k best continuations of every group
+        of `beams` rows of host logits [groups * beams, vocab], by total (normalize: scores + log-softmax; else scores +
+        logits), then beam, then token (needle_hip_beam_select).  mask: bool [vocab] or [rows, vocab], True = admitted."""
+        x = np.asarray(logits)
+        x = np.ascontiguousarray(x, dtype=np.float16 if x.dtype == np.float16 else np.float32)
+        if x.ndim != 2 or beams < 1 or x.shape[0] % beams:
+            raise ValueError("logits must be [groups * beams, vocab]")
+        rows, vocab = x.shape
+        s = None if scores is None else _f32(scores).reshape(-1)
+        f = None if finished is None else np.ascontiguousarray(np.asarray(finished).reshape(-1) != 0, dtype=np.uint8)
+        if (s is not None and s.size != rows) or (f is not None and f.size != rows):
+            raise ValueError("scores and finished need one value per row of logits")
+        words, stride = None, 0
+        if mask is not None:
+            b = np.asarray(mask, dtype=np.bool_)
+            if b.shape not in ((vocab,), (rows, vocab)):
+                raise ValueError("mask must be bool [vocab] or [rows, vocab]")
+            stride = (vocab + 31) // 32 if b.ndim == 2 else 0
+            words = np.ascontiguousarray(np.concatenate([pack_bitmask(r) for r in b.reshape(-1, vocab)]) if b.size else np.zeros(0, np.uint32))
+        groups = rows // beams
+        p = _lib.BeamParams(groups=groups, beams=beams, vocab=vocab, k=k, value=_lib.VALUE_F16 if x.dtype == np.float16 else _lib.VALUE_F32,
+                            normalize=int(bool(normalize)), row_stride=vocab, scores=None if s is None else s.ctypes.data,
+                            finished=None if f is None else f.ctypes.data, mask=None if words is None else words.ctypes.data,
+                            mask_stride=stride, end_token=end_token, reserved=0)
+        parents, tokens = np.empty((groups, k), dtype=np.uint32), np.empty((groups, k), dtype=np.uint32)
+        out, counts = np.empty((groups, k), dtype=np.float32), np.zeros(groups, dtype=np.uint32)
+        _lib.check(_lib.lib().needle_hip_beam_select(self._h, C.byref(p), x.ctypes.data, parents.ctypes.data, tokens.ctypes.data,
+                                                     out.ctypes.data, counts.ctypes.data))
+        return parents, tokens, out, counts
+
+    def beam_select_device(self, d_logits, d_scores, k: int, d_parents, d_tokens, d_out_scores, d_counts, *, beams: int,
+                           normalize: bool = True, d_mask=None, d_finished=None, end_token: int = 0, states=()) -> None:
+        """beam_select on device tensors, and the move of what the beams carry.  d_logits: float32 / float16 / bfloat16
+        [groups * beams, vocab], rows may lie apart; d_mask: int32 / uint32 words [rows, ceil(vocab / 32)] or one row of them;
+        d_finished: bool / uint8 [rows]; outputs [groups, k] (int32 / uint32, int32 / uint32, float32) and int32 / uint32
+        [groups], unused places -1 / -1 / -inf.  states: (src, dst) or (src, dst, axis) pairs of tensors whose dimension
+        `axis` (default 0) holds groups * beams rows in src and groups * k in dst; dst's rows become copies of their
+        parents' (rows of unused places stay as they were)."""
+        self._check_rows(d_logits, "d_logits")
+        rows, vocab = int(d_logits.shape[0]), int(d_logits.shape[1])
+        if beams < 1 or rows % beams:
+            raise ValueError("d_logits must be [groups * beams, vocab]")
+        groups, value = rows // beams, _value(d_logits, "d_logits")
+        if d_scores is not None:
+            self._check_flat(d_scores, "d_scores", "torch.float32", rows)
+        if d_finished is not None and str(d_finished.dtype) not in ("torch.bool", "torch.uint8"):
+            raise ValueError("d_finished must be bool or uint8")
+        if d_finished is not None:
+            self._check_flat(d_finished, "d_finished", str(d_finished.dtype), rows)
+        for t, name, size in ((d_parents, "d_parents", groups * k), (d_tokens, "d_tokens", groups * k), (d_counts, "d_counts", groups)):
+            self._check_flat(t, name, "torch.uint32" if str(t.dtype) == "torch.uint32" else "torch.int32", size)
+        self._check_flat(d_out_scores, "d_out_scores", "torch.float32", groups * k)
+        stride = 0
+        if d_mask is not None:
+            words = (vocab + 31) // 32
+            one = d_mask.reshape(1, -1) if d_mask.dim() == 1 else d_mask
+            self._check_rows(one, "d_mask", "torch.uint32" if str(d_mask.dtype) == "torch.uint32" else "torch.int32", words)
+            if int(one.shape[0]) not in (1, rows):
+                raise ValueError("d_mask must have one row, or one for every row of d_logits")
+            stride = self._stride(one) if int(one.shape[0]) == rows and rows > 1 else 0
+        arr, n_states = self._states(states, groups, beams, k)
+        self._check_device(d_logits=d_logits, d_scores=d_scores, d_mask=d_mask, d_finished=d_finished, d_parents=d_parents,
+                           d_tokens=d_tokens, d_out_scores=d_out_scores, d_counts=d_counts)
+        p = _lib.BeamParams(groups=groups, beams=beams, vocab=vocab, k=k, value=value, normalize=int(bool(normalize)),
+                            row_stride=self._stride(d_logits), scores=None if d_scores is None else d_scores.data_ptr(),
+                            finished=None if d_finished is None else d_finished.data_ptr(),
+                            mask=None if d_mask is None else d_mask.data_ptr(), mask_stride=stride, end_token=end_token, reserved=0)
+        _lib.check(_lib.lib().needle_hip_beam_select_device(self._h, C.byref(p), d_logits.data_ptr(), arr, n_states, d_parents.data_ptr(),
+                                                            d_tokens.data_ptr(), d_out_scores.data_ptr(), d_counts.data_ptr()))
+
+    def beam_reorder_device(self, d_parents, states, *, beams: int) -> None:
+        """The move of the states alone (needle_hip_beam_reorder_device), for parents [groups, k] picked elsewhere: int32 /
+        uint32 numbers below `beams`; any other number leaves its row of dst as it was."""
+        if d_parents.dim() != 2 or beams < 1:
+            raise ValueError("d_parents must be [groups, k]")
+        groups, k = int(d_parents.shape[0]), int(d_parents.shape[1])
+        self._check_flat(d_parents, "d_parents", "torch.uint32" if str(d_parents.dtype) == "torch.uint32" else "torch.int32", groups * k)
+        arr, n_states = self._states(states, groups, beams, k)
+        self._check_device(d_parents=d_parents)
+        _lib.check(_lib.lib().needle_hip_beam_reorder_device(self._h, d_parents.data_ptr(), groups, beams, k, arr, n_states))
+
+    def _states(self, states, groups: int, beams: int, k: int):
+        out = []
+        for s in states:
+            src, dst = s[0], s[1]
+            axis = s[2] if len(s) > 2 else 0
+            if src.dtype != dst.dtype or src.dim() != dst.dim() or not 0 <= axis < src.dim() or \
+                    any(a != b for i, (a, b) in enumerate(zip(src.shape, dst.shape)) if i != axis):
+                raise ValueError("a state's src and dst must differ in nothing but their rows")
+            if int(src.shape[axis]) != groups * beams or int(dst.shape[axis]) != groups * k:
+                raise ValueError(f"a state must have {groups * beams} rows in src and {groups * k} in dst")
+            for t in (src, dst):
+                if not t.is_cuda or t.device.index != self.device:
+                    raise ValueError(f"states must be tensors on device {self.device}")
+            if src.numel() == 0 or dst.numel() == 0:
+                continue
+            outer, inner, run, a, b = _state_layout(src, dst, axis)
+            out.append(_lib.BeamState(src=src.data_ptr(), dst=dst.data_ptr(), outer=outer, inner=inner, bytes=run,
+                                      src_outer_stride=a[0], src_row_stride=a[1], src_inner_stride=a[2],
+                                      dst_outer_stride=b[0], dst_row_stride=b[1], dst_inner_stride=b[2]))
+        return ((_lib.BeamState * len(out))(*out) if out else None), len(out)
 
 
 class FlatIndex:

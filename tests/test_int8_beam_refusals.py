@@ -1,0 +1,190 @@
+"""Arguments that the operators on int8 rows and beams refuse, through the C ABI and without a GPU: every check comes before
+the context or the device is touched, so a block of zeros stands for the context."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from needle_amd import _lib
+from needle_amd.index import _state_layout
+
+OK, ARG, UNSUPPORTED = _lib.OK, _lib.ERR_INVALID_ARGUMENT, _lib.ERR_UNSUPPORTED
+CTX = C.create_string_buffer(1 << 16)
+MEM = np.zeros(1 << 20, dtype=np.uint8)  # pointers into it are never followed
+BASE = (MEM.ctypes.data + 255) // 256 * 256
+
+
+def at(offset):
+    return BASE + offset
+
+
+def quantize(ctx=CTX, rows=at(0), value=0, n=4, dim=8, row_stride=8, codes=at(4096), code_stride=8, scales=at(8192)):
+    return _lib.lib().needle_hip_quantize_rows_i8_device(ctx, rows, value, n, dim, row_stride, codes, code_stride, scales)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(ctx=None), ARG), (dict(value=3), ARG), (dict(value=-1), ARG), (dict(rows=None), ARG), (dict(codes=None), ARG), (dict(scales=None), ARG),
+    (dict(row_stride=7), ARG), (dict(code_stride=7), ARG), (dict(rows=at(2)), ARG), (dict(value=1, rows=at(1)), ARG), (dict(scales=at(8193)), ARG),
+    (dict(codes=at(100)), ARG), (dict(scales=at(4096 + 8)), ARG), (dict(scales=at(0)), ARG), (dict(row_stride=1 << 61), UNSUPPORTED),
+    (dict(n=1 << 41), UNSUPPORTED), (dict(n=0), OK), (dict(n=0, rows=None, codes=None, scales=None), OK)])
+def test_quantize_rows(change, status):
+    assert quantize(**change) == status
+    if status != OK:
+        assert _lib.lib().needle_hip_last_error()
+
+
+def product(linear=False, ctx=CTX, a=at(0), a_stride=64, a_scales=at(4096), m=4, b=at(8192), b_stride=64, b_scales=at(16384), n=8, k=64,
+            bias=None, out_value=0, out=at(32768), out_stride=8, x_value=0):
+    L = _lib.lib()
+    if linear:
+        return L.needle_hip_linear_i8_device(ctx, a, x_value, a_stride, m, b, b_stride, b_scales, n, k, bias, out_value, out, out_stride)
+    return L.needle_hip_matmul_i8_device(ctx, a, a_stride, a_scales, m, b, b_stride, b_scales, n, k, bias, out_value, out, out_stride)
+
+
+@pytest.mark.parametrize("linear", (False, True))
+@pytest.mark.parametrize("change,status", [
+    (dict(ctx=None), ARG), (dict(out_value=9), ARG), (dict(k=131072, a_stride=131072, b_stride=131072), UNSUPPORTED), (dict(n=1 << 31), UNSUPPORTED),
+    (dict(a=None), ARG), (dict(b=None), ARG), (dict(b_scales=None), ARG), (dict(out=None), ARG), (dict(a_stride=63), ARG), (dict(b_stride=63), ARG),
+    (dict(out_stride=7), ARG), (dict(out=at(32769)), ARG), (dict(bias=at(50001)), ARG), (dict(b_scales=at(16385)), ARG), (dict(out=at(0)), ARG),
+    (dict(out=at(8192 + 64)), ARG), (dict(out=at(16384)), ARG), (dict(bias=at(32768)), ARG), (dict(out_stride=1 << 61), UNSUPPORTED),
+    (dict(b_stride=1 << 62), UNSUPPORTED), (dict(m=0), OK), (dict(n=0), OK)])
+def test_products(linear, change, status):
+    assert product(linear, **change) == status
+
+
+def test_products_in_their_own_way():
+    assert product(a_scales=None) == ARG and product(a_scales=at(4097)) == ARG and product(out=at(4096)) == ARG
+    assert product(True, x_value=5) == ARG and product(True, a=at(2)) == ARG
+
+
+def select(ctx=CTX, logits=at(0), parents=at(1 << 18), tokens=at((1 << 18) + 4096), scores=at((1 << 18) + 8192), counts=at((1 << 18) + 12288),
+           states=None, n_states=0, params=True, **p):
+    q = dict(groups=2, beams=3, vocab=100, k=4, value=0, normalize=1, row_stride=100, scores=None, finished=None, mask=None, mask_stride=0,
+             end_token=0, reserved=0)
+    q.update(p)
+    return _lib.lib().needle_hip_beam_select_device(ctx, C.byref(_lib.BeamParams(**q)) if params else None, logits, states, n_states, parents, tokens,
+                                                    scores, counts)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(ctx=None), ARG), (dict(params=False), ARG), (dict(value=4), ARG), (dict(reserved=1), ARG), (dict(k=257), UNSUPPORTED),
+    (dict(beams=1025), UNSUPPORTED), (dict(beams=1024, vocab=1 << 22, row_stride=1 << 22), UNSUPPORTED),
+    (dict(groups=1 << 30, beams=2), UNSUPPORTED), (dict(groups=1 << 30, k=2, beams=1), UNSUPPORTED), (dict(logits=None), ARG), (dict(parents=None), ARG),
+    (dict(tokens=None), ARG), (dict(counts=None), ARG), (dict(row_stride=99), ARG), (dict(mask=at(4096 * 9), mask_stride=3), ARG),
+    (dict(finished=at(4096 * 9), end_token=100), ARG), (dict(logits=at(2)), ARG), (dict(value=2, logits=at(1)), ARG), (dict(mask=at(4096 * 9 + 2)), ARG),
+    (dict(counts=at(1 << 18)), ARG), (dict(parents=at(400)), ARG), (dict(row_stride=1 << 62), UNSUPPORTED), (dict(groups=0), OK),
+    (dict(n_states=1), ARG), (dict(n_states=257, states=(_lib.BeamState * 257)()), UNSUPPORTED)])
+def test_select(change, status):
+    assert select(**change) == status
+
+
+def state(**change):
+    """groups 2, beams 3, k 4: six rows of two runs of 32 bytes become eight."""
+    s = dict(src=at(1 << 16), dst=at(1 << 17), outer=1, inner=2, bytes=32, src_outer_stride=0, src_row_stride=100, src_inner_stride=40,
+             dst_outer_stride=0, dst_row_stride=100, dst_inner_stride=40)
+    s.update(change)
+    return s
+
+
+def reorder(*states, ctx=CTX, parents=at(0), groups=2, beams=3, k=4):
+    arr = (_lib.BeamState * len(states))(*[_lib.BeamState(**s) for s in states])
+    return _lib.lib().needle_hip_beam_reorder_device(ctx, parents, groups, beams, k, arr, len(states))
+
+
+@pytest.mark.parametrize("states,status", [
+    ([state(src=None)], ARG), ([state(dst=None)], ARG), ([state(dst_inner_stride=31)], ARG), ([state(dst_row_stride=71)], ARG),
+    ([state(outer=3, dst_outer_stride=300)], ARG), ([state(dst_row_stride=0)], ARG), ([state(dst=at((1 << 16) + 200))], ARG),
+    ([state(dst=at(1 << 16))], ARG), ([state(), state(src=at(1 << 15))], ARG), ([state(), state(src=at(1 << 17), dst=at(1 << 18))], ARG),
+    ([state(dst_row_stride=1 << 61)], UNSUPPORTED), ([state(src_row_stride=1 << 61)], UNSUPPORTED), ([], OK),
+    ([state(inner=0, src=None, dst=None)], None)])
+def test_states(states, status):
+    got = reorder(*states)
+    assert got == status if status is not None else got in (_lib.ERR_HIP, _lib.OK)  # nothing to refuse: only the device is missing
+    assert reorder(state(), ctx=None) == ARG and reorder(state(), parents=None) == ARG
+    assert reorder(state(), groups=0) == OK and reorder(state(), k=0) == OK
+
+
+def test_state_layouts():
+    import torch
+
+    src, dst = torch.zeros(6, 3, 20, 64, dtype=torch.bfloat16), torch.zeros(8, 3, 20, 64, dtype=torch.bfloat16)
+    assert _state_layout(src, dst, 0) == (1, 1, 3 * 20 * 64 * 2, (0, 7680, 0), (0, 7680, 0))
+    assert _state_layout(src[:, :, :5], dst[:, :, :5], 0) == (1, 3, 640, (0, 7680, 2560), (0, 7680, 2560))
+    assert _state_layout(src[:, :1, :, 7:8], dst[:, :1, :, 7:8], 0) == (1, 20, 2, (0, 7680, 128), (0, 7680, 128))
+    a, b = torch.zeros(2, 5, 6, 9), torch.zeros(2, 5, 8, 9)
+    assert _state_layout(a, b, 2) == (10, 1, 36, (216, 36, 0), (288, 36, 0))
+    with pytest.raises(ValueError):
+        _state_layout(a[:, :2], b[:, :2], 2)  # two dimensions before the rows that do not fold
+    with pytest.raises(ValueError):
+        _state_layout(src[:, :2, :5, ::2], dst[:, :2, :5, ::2], 0)
+
+
+def test_python_checks():
+    """The object layer refuses before it calls the library."""
+    import torch
+
+    from needle_amd import Context
+
+    c = Context.__new__(Context)
+    c.device, c._h = 0, C.c_void_p()
+    f, i8 = torch.zeros(4, 8), torch.zeros(4, 8, dtype=torch.int8)
+    s = torch.zeros(4)
+    bad = [lambda: c.quantize_rows_device(f.double(), i8, s), lambda: c.quantize_rows_device(f, i8.int(), s), lambda: c.quantize_rows_device(f.T, i8, s),
+           lambda: c.quantize_rows_device(f, i8, s[:3]), lambda: c.quantize_rows_device(f, i8, s), lambda: c.quantize_rows_device(f[0].expand(4, 8), i8, s),
+           lambda: c.quantize_rows(np.zeros(4, np.float32)),
+           lambda: c.matmul_i8_device(i8, s, i8[:, :4], s, torch.zeros(4, 4)), lambda: c.matmul_i8_device(i8, s, i8, s, torch.zeros(4, 5)),
+           lambda: c.matmul_i8_device(f, s, i8, s, torch.zeros(4, 4)), lambda: c.matmul_i8_device(i8, s, i8, s, torch.zeros(4, 4)),
+           lambda: c.matmul_i8_device(i8, s, i8, s, torch.zeros(4, 4, dtype=torch.int32)), lambda: c.linear_i8_device(i8, i8, s, torch.zeros(4, 4)),
+           lambda: c.matmul_i8(np.zeros((4, 8)), np.zeros(4), np.zeros((4, 8), np.int8), np.zeros(4)),
+           lambda: c.matmul_i8(np.zeros((4, 8), np.int8), np.zeros(3), np.zeros((4, 8), np.int8), np.zeros(4)),
+           lambda: c.matmul_i8(np.zeros((4, 8), np.int8), np.zeros(4), np.zeros((4, 9), np.int8), np.zeros(4)),
+           lambda: c.beam_select(np.zeros((4, 8)), None, 2, beams=3), lambda: c.beam_select(np.zeros((4, 8)), np.zeros(3), 2, beams=2),
+           lambda: c.beam_select(np.zeros((4, 8)), None, 2, beams=2, mask=np.ones(7, bool))]
+    i = torch.zeros(2, 3, dtype=torch.int32)
+    n = torch.zeros(2, dtype=torch.int32)
+
+    def sel(logits=f, scores=s, k=3, p=i, t=i, o=torch.zeros(2, 3), cnt=n, beams=2, **kw):
+        return lambda: c.beam_select_device(logits, scores, k, p, t, o, cnt, beams=beams, **kw)
+
+    bad += [sel(), sel(beams=3), sel(beams=0), sel(logits=f.double()), sel(scores=s[:2]), sel(p=i.long()), sel(cnt=torch.zeros(3, dtype=torch.int32)),
+            sel(o=torch.zeros(2, 3).half()), sel(d_mask=torch.zeros(4, 2, dtype=torch.int32)), sel(d_mask=torch.zeros(2, 1, dtype=torch.int32)),
+            sel(d_finished=torch.zeros(4)), sel(d_finished=torch.zeros(3, dtype=torch.bool)), sel(states=[(f, torch.zeros(6, 8))]),
+            sel(states=[(f, torch.zeros(5, 8))]), sel(states=[(f, torch.zeros(6, 9))]), sel(states=[(f, torch.zeros(6, 8).half())])]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_structs_and_constants_mirror_the_header():
+    import os
+    import re
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    header = open(os.path.join(root, "include", "needle_hip.h")).read()
+    rust = open(os.path.join(root, "bindings", "rust", "needle-hip-sys", "src", "lib.rs")).read()
+
+    def names(text, opener, pattern):
+        body = text[text.index(opener):]
+        body = re.sub(r"/\*.*?\*/|//[^\n]*", "", body[body.index("{") + 1: body.index("}")], flags=re.S)
+        return re.findall(pattern, body)
+
+    for struct, mirror in (("needle_beam_params", _lib.BeamParams), ("needle_beam_state", _lib.BeamState)):
+        fields = [n for line in names(header, f"typedef struct {struct}", r"([^;]+);") for n in re.findall(r"([a-z_0-9]+)\s*(?:,|$)", line.strip())]
+        assert [n for n, _ in mirror._fields_] == fields
+        assert names(rust, f"pub struct {struct}", r"pub\s+([a-z_0-9]+)\s*:") == fields
+    assert C.sizeof(_lib.BeamParams) == 72 and C.sizeof(_lib.BeamState) == 88
+    for name, value in re.findall(r"\b(NEEDLE_VALUE_[A-Z0-9]+)\s*=\s*(\d+)", header):
+        assert f"pub const {name}: c_int = {value};" in rust and getattr(_lib, name[len("NEEDLE_"):]) == int(value)
+
+
+def test_build_rs_compiles_the_operators_as_the_makefile_does():
+    import os
+    import re
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    mk = open(os.path.join(root, "needle_amd", "csrc", "Makefile")).read()
+    rs = open(os.path.join(root, "bindings", "rust", "needle-hip-sys", "build.rs")).read()
+    objs = re.search(r"^OPERATOR_OBJS := (.*)$", mk, flags=re.M).group(1).split()
+    flags = re.search(r"^OPERATOR_FLAGS := (.*)$", mk, flags=re.M).group(1).split()
+    assert re.findall(r'"([^"]+)"', re.search(r"const OPERATOR_SOURCES[^=]*=([^;]*);", rs).group(1)) == [o.replace(".o", ".hip") for o in objs]
+    assert re.findall(r'"([^"]+)"', re.search(r"const OPERATOR_FLAGS[^=]*=([^;]*);", rs).group(1)) == flags

@@ -16,7 +16,8 @@ SCALARS = {"needle_hip_status": "c_int", "int": "c_int", "needle_metric": "c_int
            "uint64_t": "u64", "uint32_t": "u32", "uint16_t": "u16", "uint8_t": "u8", "float": "f32", "double": "f64", "void": "c_void",
            "char": "c_char", "needle_hip_ctx": "needle_hip_ctx", "needle_hip_index": "needle_hip_index",
            "needle_hip_comm": "needle_hip_comm", "needle_search_params": "needle_search_params",
-           "needle_hip_metrics": "needle_hip_metrics"}
+           "needle_hip_metrics": "needle_hip_metrics", "int8_t": "i8", "needle_beam_params": "needle_beam_params",
+           "needle_beam_state": "needle_beam_state"}
 
 
 def prototypes():
