@@ -7,8 +7,11 @@
 // keeps, per piece of a row, its maximum, its sum of exponentials and its k largest logits; a second, small kernel joins the
 // pieces of a group.  The pass is bound by the bytes of the logits.
 //
-// Picks are whole numbers and two beams' totals may lie a rounding apart, so whatever decides between beams is held in
-// 64 bits: the exponentials, their sums, the totals.  (f64 fused multiply-adds issue at the rate of f32 ones here.)
+// Picks are whole numbers and two beams' totals may lie a rounding apart, so what decides between beams is held in 64 bits:
+// the totals, the sums, and the exponentials of the logits that may be picked -- they are the large terms of a sum.  The
+// many small terms are taken in f32 by a polynomial whose error (3e-8 of a term, mean 1.3e-9) averages out over them: an
+// f64 instruction takes twice the cycles of an f32 one here, and eight f64 ones per logit bound the kernel (73 us for 64 x 8
+// rows of 131072 bf16 logits).
 #include "nh_values.h"
 
 namespace nh {
@@ -16,24 +19,42 @@ namespace nh {
 constexpr uint32_t BEAM_K_MAX = 256, BEAMS_MAX = 1024;
 constexpr uint32_t PIECE_THREADS = 256;
 
-// ---- exponential of x <= 0 in 64 bits -------------------------------------------------------
-// exp x = 2^n exp f with n = rint(x / ln 2), |f| <= ln 2 / 2, and exp f by its Taylor series to f^9: the first term left
-// out is below 2^-37 * 2^-1.5 / 10! ~ 7e-12 of the result.  Below -800 the result is 0 (as exp's own, from -746 on).
-__device__ inline double exp_below0(double x) {
-    x = fmax(x, -800.0);
-    const double n = rint(x * 1.4426950408889634074);
-    const double f = __builtin_fma(n, -0.69314718055994530942, x);
-    double p = 2.7557319223985893e-06;  // 1 / 9!
-    p = __builtin_fma(p, f, 2.4801587301587302e-05);
-    p = __builtin_fma(p, f, 1.9841269841269841e-04);
-    p = __builtin_fma(p, f, 1.3888888888888889e-03);
-    p = __builtin_fma(p, f, 8.3333333333333333e-03);
-    p = __builtin_fma(p, f, 4.1666666666666667e-02);
-    p = __builtin_fma(p, f, 1.6666666666666667e-01);
-    p = __builtin_fma(p, f, 0.5);
-    p = __builtin_fma(p, f, 1.0);
-    p = __builtin_fma(p, f, 1.0);
-    return ldexp(p, (int)n);
+// ---- exponential of x <= 64 in 64 bits -------------------------------------------------------
+// exp x = 2^n 2^f with n the whole number nearest to x / ln 2 (found by adding 1.5 * 2^52, which leaves it in the low
+// bits of the sum) and 2^f, |f| <= 1/2, by a polynomial of degree 7 that equals it at the eight Chebyshev nodes: at most
+// 5.6e-11 of the result off, with changing sign.  Below -700 the result is that of -700, 1e-304: nothing beside a 1.
+__device__ inline double exp64(double x) {
+    constexpr double ONE_AND_A_HALF = 6755399441055744.0, PER_LN2 = 1.4426950408889634074;
+    x = fmax(x, -700.0);
+    const double s = __builtin_fma(x, PER_LN2, ONE_AND_A_HALF);
+    const double f = __builtin_fma(x, PER_LN2, -(s - ONE_AND_A_HALF));
+    double p = 0x1.00c0e4e15189cp-16;
+    p = __builtin_fma(p, f, 0x1.446c79efd4834p-13);
+    p = __builtin_fma(p, f, 0x1.5d877598350dep-10);
+    p = __builtin_fma(p, f, 0x1.3b29d8bb0b97ep-7);
+    p = __builtin_fma(p, f, 0x1.c6b08da70cce3p-5);
+    p = __builtin_fma(p, f, 0x1.ebfbe0aa03df0p-3);
+    p = __builtin_fma(p, f, 0x1.62e42fef9cc69p-1);
+    p = __builtin_fma(p, f, 0x1.ffffffffa7135p-1);
+    return __hiloint2double(__double2hiint(p) + (__double2loint(s) << 20), __double2loint(p));
+}
+
+// exp x in units of 2^nref, for |x| < 2^20 and x / ln 2 - nref > -120, in f32: 2^f by a polynomial of degree 6 through the
+// seven Chebyshev nodes of |f| <= 1/2.  `shift` = 1.5 * 2^23 - nref, so that the sum with x / ln 2 holds n - nref in its low
+// bits; the two multiply-adds keep f to 2^-26 however large n is.
+__device__ inline float exp32_scaled(float x, float shift) {
+    constexpr float HI = 0x1.715476p+0f, LO = 0x1.4ae0cp-26f;  // 1 / ln 2
+    const float s = __builtin_fmaf(x, HI, shift), n = s - shift;
+    float f = __builtin_fmaf(x, HI, -n);
+    f = __builtin_fmaf(x, LO, f);
+    float p = 0x1.444p-13f;
+    p = __builtin_fmaf(p, f, 0x1.5f48cp-10f);
+    p = __builtin_fmaf(p, f, 0x1.3b2a1cp-7f);
+    p = __builtin_fmaf(p, f, 0x1.c6aeccp-5f);
+    p = __builtin_fmaf(p, f, 0x1.ebfbep-3f);
+    p = __builtin_fmaf(p, f, 0x1.62e43p-1f);
+    p = __builtin_fmaf(p, f, 1.0f);
+    return __uint_as_float(__float_as_uint(p) + (__float_as_uint(s) << 23));
 }
 
 // order-preserving whole number of a double (-0 as +0); 0 for what is never offered (-inf, NaN)
@@ -46,7 +67,7 @@ __device__ inline double of_order64(uint64_t o) {
     return __longlong_as_double((long long)((o >> 63) ? (o & 0x7fffffffffffffffull) : ~o));
 }
 
-// ---- across a workgroup of 4 waves ---------------------------------------------------------
+// ---- across a workgroup ---------------------------------------------------------
 __device__ inline uint32_t wave_max(uint32_t v) {
     for (int o = 32; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
     return v;
@@ -55,8 +76,8 @@ __device__ inline double wave_sum(double v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
-// The k-th largest of the 64 * PER values of `maxima` (zeros among them count as absent: 0 if there are fewer), cut to
-// its upper 20 bits: at least k of the values are >= the result.  Every wave computes it for itself.
+// By one wave: the k-th largest of the 64 * PER values of `maxima` (zeros among them count as absent: 0 if there are
+// fewer), cut to its upper 20 bits: at least k of the values are >= the result.
 template <int PER>
 __device__ inline uint32_t kth_largest(const uint32_t* maxima, uint32_t k, uint32_t lane) {
     uint32_t v[PER], t = 0;
@@ -71,13 +92,33 @@ __device__ inline uint32_t kth_largest(const uint32_t* maxima, uint32_t k, uint3
     }
     return t;
 }
-// Sum of one count per thread over the workgroup; `slot` is LDS of 2 x 4 words that two calls in a row use in turn.
+// How many of the first n values of `list` lie above each of `mine`; the list is read eight at a time and ends in zeros up
+// to the next multiple of eight.
+template <int MINE>
+__device__ inline void count_above(const uint64_t* list, uint32_t n, const uint64_t (&mine)[MINE], uint32_t (&above)[MINE]) {
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) above[i] = 0;
+    for (uint32_t j = 0; j < n; j += 8) {
+        uint64_t o[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) o[u] = list[j + u];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) above[i] += o[u] > mine[i];
+    }
+}
+// Sum of one count per thread over the workgroup's WAVES; `slot` is LDS of 2 x WAVES words that two calls in a row use in
+// turn.
+template <int WAVES>
 __device__ inline uint32_t block_count(uint32_t mine, uint32_t* slot, uint32_t turn) {
     for (int o = 32; o; o >>= 1) mine += (uint32_t)__shfl_xor((int)mine, o);
-    uint32_t* s = slot + (turn & 1) * 4;
+    uint32_t* s = slot + (turn & 1) * WAVES;
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = mine;
     __syncthreads();
-    return s[0] + s[1] + s[2] + s[3];
+    uint32_t all = 0;
+    for (int w = 0; w < WAVES; ++w) all += s[w];
+    return all;
 }
 
 struct BeamParams {
@@ -86,9 +127,12 @@ struct BeamParams {
     const uint8_t* finished;  // [rows] or null
     const uint32_t* mask;     // or null
     uint64_t row_stride, mask_stride;
-    uint32_t rows, groups, beams, vocab, k, pieces, end_token, normalize;
+    uint32_t rows, groups, beams, vocab, k, end_token;
+    uint32_t pieces, chunks_per_piece;  // of a row
+    uint32_t len;                           // entries of a piece's list, >= k
+    uint32_t per_row_magic, per_row_shift;  // i / (pieces * len) = (i * magic) >> (31 + shift) for i < 2^31
     // per (row, piece)
-    uint64_t* list;   // [rows][pieces][k]: order of the logit << 32 | ~token, best first, 0 behind the last
+    uint64_t* list;   // [rows][pieces][len]: order of the logit << 32 | ~token in any order, 0 behind the last
     double* sum;      // [rows][pieces] sum of exp(x - peak)
     float* peak;      // [rows][pieces] largest admitted logit; -inf: none; NaN: a NaN among them
     uint32_t* out_parents;
@@ -97,153 +141,293 @@ struct BeamParams {
     uint32_t* out_counts;
 };
 
-// One piece (PIECE_THREADS * EACH logits) of one row, held in registers.  GROUPS maxima per thread narrow the piece to
-// the logits that can be among its k largest: the k-th largest of all these maxima is reached by k logits.
-template <typename V, int EACH, int GROUPS>
+// One piece of one row: chunks_per_piece chunks of PIECE_THREADS * EACH logits, each held in registers while the next one is
+// under way.  A list in LDS keeps what can be among the piece's k largest.  What reaches the list has to reach a bound: the
+// k-th largest of GROUPS running maxima per thread, which k logits reach; it is found again after 1, 2, 4, 8, ... chunks, so
+// that about k log2(chunks) logits are listed in all.  Which logits a thread adds up, and in which order, follows from the
+// places and values of its row alone: equal rows have equal sums.
+template <typename V, int EACH, int GROUPS, bool NORMALIZE, bool MASKED>
 __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p) {
-    constexpr int WIDE = 16 / V::size, LOADS = EACH / WIDE, PIECE = PIECE_THREADS * EACH, CAP = 1024;
+    constexpr int WIDE = 16 / V::size, LOADS = EACH / WIDE, CAP = 1024, MINE = CAP / PIECE_THREADS;
+    constexpr uint32_t CHUNK = PIECE_THREADS * EACH, LOWEST = 0x00800000u;  // LOWEST: order of the lowest finite f32
+    constexpr double LN2 = 0.69314718055994530942;
     __shared__ uint32_t s_max[PIECE_THREADS * GROUPS];
-    __shared__ uint64_t s_list[CAP];
+    __shared__ __align__(16) uint64_t s_list[CAP + 8];
     __shared__ double s_sum[4];
-    __shared__ uint32_t s_top[4], s_nan, s_n, s_cnt[8];
+    __shared__ float s_top[4];
+    __shared__ uint32_t s_nan, s_add[3], s_bound, s_fill;
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const uint32_t row = blockIdx.x / p.pieces, piece = blockIdx.x % p.pieces;
     const size_t at = (size_t)row * p.pieces + piece;
-    uint64_t* list = p.list + at * p.k;
+    uint64_t* list = p.list + at * p.len;
     const bool ended = p.finished && p.finished[row];
     const float start = p.scores ? p.scores[row] : 0.0f;
     if (ended || !(start > -__builtin_inff())) {  // nothing of this row is looked at
-        for (uint32_t i = t; i < p.k; i += PIECE_THREADS)
+        for (uint32_t i = t; i < p.len; i += PIECE_THREADS)
             list[i] = ended && piece == 0 && i == 0 ? ((uint64_t)f2ord(0.0f) << 32) | (uint32_t)~p.end_token : 0;
         if (t == 0) { p.sum[at] = 0.0; p.peak[at] = -__builtin_inff(); }
         return;
     }
-    if (t == 0) { s_nan = 0; s_n = 0; }
+    if (t == 0) { s_nan = 0; s_add[0] = 0; s_add[1] = 0; }
     const typename V::bits* x = (const typename V::bits*)p.logits + (uint64_t)row * p.row_stride;
-    const uint32_t* mask = p.mask ? p.mask + (uint64_t)row * p.mask_stride : nullptr;
-    const uint32_t first = piece * PIECE;
-    // order of every logit (0: not admitted, -inf or NaN)
-    uint32_t key[EACH];
+    const uint32_t* mask = MASKED ? p.mask + (uint64_t)row * p.mask_stride : nullptr;
+    const uint32_t first = piece * p.chunks_per_piece * CHUNK;
+    const uint32_t behind = (uint32_t)min((uint64_t)p.vocab, (uint64_t)first + (uint64_t)p.chunks_per_piece * CHUNK);
+
+    u32x4 raw[LOADS];
+    uint32_t bits[LOADS];
+    auto load = [&](uint32_t chunk0) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const uint32_t tok = chunk0 + (j * PIECE_THREADS + t) * WIDE;
+            if (tok + WIDE <= p.vocab) {
+                raw[j] = *(const u32x4_any*)(x + tok);
+            } else {  // -inf behind the end
+                typename V::bits one[WIDE];
+#pragma unroll
+                for (int w = 0; w < WIDE; ++w) one[w] = tok + w < p.vocab ? x[tok + w] : V::round(-__builtin_inff());
+                __builtin_memcpy(&raw[j], one, 16);
+            }
+            if (MASKED) bits[j] = tok < p.vocab ? mask[tok >> 5] >> (tok & 31) : 0;  // WIDE divides 32
+        }
+    };
+    load(first);
+
+    uint32_t n = 0;      // entries of the list
+    float bound = 0.0f;  // a logit below it is not among the k largest
+    float run[GROUPS];   // largest logits of this thread so far
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) run[g] = -__builtin_inff();
+    // the thread's sum of exponentials, in units of exp(unit) = 2^nref where the f32 path applies
+    double sum = 0.0, unit = 0.0;
+    float ref = -__builtin_inff(), shift = 0.0f;
     bool nan = false;
+    uint32_t slot = 0;
+
+    // bound := the k-th largest running maximum
+    auto raise = [&] {
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-        const uint32_t tok = first + (j * PIECE_THREADS + t) * WIDE;
-        u32x4 raw = {0, 0, 0, 0};
-        typename V::bits one[WIDE];
-        if (tok + WIDE <= p.vocab) {
-            raw = *(const u32x4_any*)(x + tok);
-            __builtin_memcpy(one, &raw, 16);
-        } else {
-#pragma unroll
-            for (int w = 0; w < WIDE; ++w) one[w] = tok + w < p.vocab ? x[tok + w] : (typename V::bits)0;
+        for (int g = 0; g < GROUPS; ++g) s_max[g * PIECE_THREADS + t] = run[g] > -__builtin_inff() ? f2ord(run[g] + 0.0f) : 0;
+        __syncthreads();
+        if (wave == 0) {
+            const uint32_t kth = kth_largest<4 * GROUPS>(s_max, p.k, lane);
+            if (lane == 0) s_bound = max(kth, LOWEST);
         }
-        const uint32_t bits = mask ? (tok < p.vocab ? mask[tok >> 5] >> (tok & 31) : 0) : ~0u;  // WIDE divides 32
+        __syncthreads();
+        return ord2f(s_bound);
+    };
+    // the list cut to its k largest, by counting; true if it held more
+    auto cut = [&] {
+        if (n <= p.k) return false;
+        uint64_t mine[MINE];
+        uint32_t rank[MINE];
 #pragma unroll
-        for (int w = 0; w < WIDE; ++w) {
-            const bool in = tok + w < p.vocab && ((bits >> w) & 1);
-            const float f = V::widen(one[w]);
-            nan |= in && f != f;
-            key[j * WIDE + w] = in && f > -__builtin_inff() ? f2ord(f + 0.0f) : 0;
+        for (int i = 0; i < MINE; ++i) mine[i] = t + i * PIECE_THREADS < n ? s_list[t + i * PIECE_THREADS] : 0;
+        if (t < 8) s_list[n + t] = 0;
+        __syncthreads();
+        count_above<MINE>(s_list, n, mine, rank);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < MINE; ++i)
+            if (mine[i] && rank[i] < p.k) s_list[rank[i]] = mine[i];
+        __syncthreads();
+        n = p.k;
+        return true;
+    };
+
+    uint32_t done = 0;
+    for (uint32_t chunk0 = first;; chunk0 += CHUNK) {
+        float v[EACH];
+        bool here = false;  // a NaN in this chunk
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            typename V::bits one[WIDE];
+            __builtin_memcpy(one, &raw[j], 16);
+#pragma unroll
+            for (int w = 0; w < WIDE; ++w) {
+                const float f = V::widen(one[w]);
+                v[j * WIDE + w] = !MASKED || ((bits[j] >> w) & 1) ? f : -__builtin_inff();
+                here |= v[j * WIDE + w] != v[j * WIDE + w];
+            }
         }
+        if (__any(here)) {
+            nan |= here;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) v[e] = v[e] != v[e] ? -__builtin_inff() : v[e];
+        }
+        const bool more = behind - chunk0 > CHUNK;
+        if (more) load(chunk0 + CHUNK);
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            float m = -__builtin_inff();
+#pragma unroll
+            for (int e = g * (EACH / GROUPS); e < (g + 1) * (EACH / GROUPS); ++e) m = fmaxf(m, v[e]);
+            top = fmaxf(top, m);
+            run[g] = fmaxf(run[g], m);
+        }
+        ++done;
+        if ((done & (done - 1)) == 0) {
+            const float b = raise();
+            bound = done == 1 ? b : fmaxf(bound, b);
+        }
+        const float listed = bound;
+        const bool any = __any(top >= listed);
+        // the logits that reach `least` go behind the list's n entries: one place per wave, then one per logit; how many
+        auto append = [&](float least) {
+            if (__any(top >= least)) {
+                uint32_t cnt = 0;
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) cnt += (uint32_t)__popcll(__ballot(v[e] >= least));
+                uint32_t base = 0;
+                if (lane == 0) base = atomicAdd(&s_add[slot], cnt);
+                base = n + (uint32_t)__builtin_amdgcn_readfirstlane((int)base);
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) {
+                    const uint64_t who = __ballot(v[e] >= least);
+                    if (who) {
+                        const uint32_t i = base + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+                        if (v[e] >= least && i < CAP) {
+                            const uint32_t tok = chunk0 + ((e / WIDE) * PIECE_THREADS + t) * WIDE + e % WIDE;
+                            s_list[i] = ((uint64_t)f2ord(v[e] + 0.0f) << 32) | (uint32_t)~tok;
+                        }
+                        base += (uint32_t)__popcll(who);
+                    }
+                }
+            }
+            // three counters in turn: the next one was last read before the barrier before this one
+            if (t == 0) s_add[slot == 2 ? 0 : slot + 1] = 0;
+            __syncthreads();
+            const uint32_t add = s_add[slot];
+            slot = slot == 2 ? 0 : slot + 1;
+            return add;
+        };
+        uint32_t add = append(listed);
+        if (n + add > CAP) {
+            // Large logits that come late in the row: this chunk raises the bound itself.  If thousands still reach it
+            // (equal ones, or an order that puts all large ones into few threads), one logit of every thread at a time
+            // goes to the list, which is cut back as it fills.
+            bound = fmaxf(bound, raise());
+            add = 0;
+            if (t == 0) s_fill = n;
+            __syncthreads();
+#pragma unroll 1
+            for (uint32_t e0 = 0; e0 < EACH; ++e0) {
+                float y = -__builtin_inff();
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) y = e0 == (uint32_t)e ? v[e] : y;
+                if (y >= bound) {
+                    const uint32_t tok = chunk0 + ((e0 / WIDE) * PIECE_THREADS + t) * WIDE + e0 % WIDE;
+                    s_list[atomicAdd(&s_fill, 1u)] = ((uint64_t)f2ord(y + 0.0f) << 32) | (uint32_t)~tok;
+                }
+                __syncthreads();
+                n = s_fill;
+                __syncthreads();
+                if (n > CAP - PIECE_THREADS && cut()) {
+                    bound = fmaxf(bound, ord2f((uint32_t)(s_list[n - 1] >> 32)));
+                    if (t == 0) s_fill = n;
+                    __syncthreads();
+                }
+            }
+            // the k-th's equals in later chunks come behind it: the next f32
+            if (cut()) bound = fmaxf(bound, ord2f((uint32_t)(s_list[n - 1] >> 32) + 1));
+        }
+        n += add;
+        if (NORMALIZE && top > -__builtin_inff()) {
+            if (!(top - ref <= 20.0f)) {  // ref is -inf at first
+                const bool started = ref > -__builtin_inff();
+                const double was = unit;
+                ref = top;
+                const float nref = rintf(ref * 1.44269504f);
+                shift = 12582912.0f - nref;  // 1.5 * 2^23
+                unit = fabsf(ref) < 0x1p20f ? (double)nref * LN2 : (double)ref;
+                sum = started ? sum * exp64(was - unit) : 0.0;
+            }
+            const bool small = fabsf(ref) < 0x1p20f;
+            // In 64 bits, one logit of every thread at a time: what the list got, or all of them where f32 has no digits left.
+            if (any || __any(!small)) {
+                uint32_t left = 0;
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) left |= v[e] >= (small ? listed : -3.40282347e+38f) ? 1u << e : 0;
+#pragma unroll 1
+                while (__any(left != 0)) {
+                    const uint32_t e0 = left ? (uint32_t)__builtin_ctz(left) : ~0u;
+                    float y = -__builtin_inff();
+#pragma unroll
+                    for (int e = 0; e < EACH; ++e)
+                        if (e0 == (uint32_t)e) {
+                            y = v[e];
+                            v[e] = -__builtin_inff();
+                        }
+                    if (left) sum += exp64((double)y - unit);
+                    left &= left - 1;
+                }
+            }
+            const float least = ref - 80.0f;  // e^-80 beside a term of 1 is nothing
+            float part = 0.0f;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                part += exp32_scaled(fmaxf(v[e], least), shift);
+                if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: more in flight cost registers, and waves
+            }
+            if (small) sum += (double)part;
+        }
+        if (!more) break;
     }
-    uint32_t top = 0;
+    if (NORMALIZE) {
+        float m = run[0];
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int e = g * (EACH / GROUPS); e < (g + 1) * (EACH / GROUPS); ++e) m = max(m, key[e]);
-        s_max[g * PIECE_THREADS + t] = m;
-        top = max(top, m);
-    }
-    top = wave_max(top);
-    if (lane == 0) s_top[wave] = top;
-    __syncthreads();
-    if (nan) s_nan = 1;
-    top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
-    const float peak = top ? ord2f(top) : -__builtin_inff();
-    double sum = 0.0;
-    if (p.normalize && top) {
-#pragma unroll
-        for (int e = 0; e < EACH; ++e)
-            if (key[e]) sum += exp_below0((double)ord2f(key[e]) - (double)peak);
+        for (int g = 1; g < GROUPS; ++g) m = fmaxf(m, run[g]);
+        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        if (lane == 0) s_top[wave] = m;
+        if (nan) s_nan = 1;
+        __syncthreads();
+        m = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+        sum = ref > -__builtin_inff() ? sum * exp64(unit - (double)m) : 0.0;
         sum = wave_sum(sum);
         if (lane == 0) s_sum[wave] = sum;
-    }
-    // the logits at or above the pivot
-    const uint32_t pivot = max(kth_largest<4 * GROUPS>(s_max, p.k, lane), 1u);
-#pragma unroll
-    for (int e = 0; e < EACH; ++e)
-        if (key[e] >= pivot) {
-            const uint32_t i = atomicAdd(&s_n, 1u);
-            const uint32_t tok = first + ((e / WIDE) * PIECE_THREADS + t) * WIDE + e % WIDE;
-            if (i < CAP) s_list[i] = ((uint64_t)key[e] << 32) | (uint32_t)~tok;
-        }
-    __syncthreads();
-    uint32_t n = s_n;
-    if (t == 0) {
-        p.sum[at] = p.normalize && top ? (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]) : 0.0;
-        p.peak[at] = s_nan ? __uint_as_float(0x7fc00000u) : peak;
-    }
-    if (n > CAP) {
-        // thousands of equal logits, or an order that puts all large ones into few threads: the k-th largest logit bit by
-        // bit, then the lowest places among those that equal it
-        uint32_t turn = 0, kth = 0, below = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t cand = kth | (1u << bit);
-            uint32_t c = 0;
-#pragma unroll
-            for (int e = 0; e < EACH; ++e) c += key[e] >= cand;
-            if (block_count(c, s_cnt, turn++) >= p.k) kth = cand;
-        }
-        uint32_t c = 0;
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) c += key[e] > kth;
-        const uint32_t need = p.k - block_count(c, s_cnt, turn++);  // >= 1 of those equal to it
-        for (int bit = 13; bit >= 0; --bit) {  // the largest place that fewer than `need` of them lie below
-            const uint32_t cand = below | (1u << bit);
-            c = 0;
-#pragma unroll
-            for (int e = 0; e < EACH; ++e) c += key[e] == kth && ((e / WIDE) * PIECE_THREADS + t) * WIDE + e % WIDE < cand;
-            if (block_count(c, s_cnt, turn++) < need) below = cand;
-        }
         __syncthreads();
-        if (t == 0) s_n = 0;
+        if (t == 0) {
+            p.sum[at] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+            p.peak[at] = s_nan ? __uint_as_float(0x7fc00000u) : m;
+        }
+    }
+    if (n > p.len) {  // what the last bound lets through; the k largest by counting if that is still too much
+        const float b = raise();
+        const uint64_t least = (uint64_t)f2ord(fmaxf(bound, b)) << 32;
+        uint64_t mine[MINE];
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) mine[i] = t + i * PIECE_THREADS < n ? s_list[t + i * PIECE_THREADS] : 0;
+        if (t == 0) s_fill = 0;
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-            const uint32_t place = ((e / WIDE) * PIECE_THREADS + t) * WIDE + e % WIDE;
-            if (key[e] > kth || (key[e] == kth && place <= below))
-                s_list[atomicAdd(&s_n, 1u)] = ((uint64_t)key[e] << 32) | (uint32_t)~(first + place);
-        }
+        for (int i = 0; i < MINE; ++i)
+            if (mine[i] >= least) s_list[atomicAdd(&s_fill, 1u)] = mine[i];
         __syncthreads();
-        n = s_n;  // k
+        n = s_fill;
+        if (n > p.len) cut();
     }
-    // their order by counting: the entries are all different
-    for (uint32_t i = t; i < n; i += PIECE_THREADS) {
-        const uint64_t mine = s_list[i];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; ++j) rank += s_list[j] > mine;
-        if (rank < p.k) list[rank] = mine;
-    }
-    for (uint32_t i = n + t; i < p.k; i += PIECE_THREADS) list[i] = 0;
+    for (uint32_t i = t; i < p.len; i += PIECE_THREADS) list[i] = i < n ? s_list[i] : 0;
 }
 
-// One group: the logs of its rows' sums, the totals of what the pieces listed, and the k best of them.
-template <int GROUPS>
-__global__ __launch_bounds__(256) void beam_join_kernel(BeamParams p) {
+// One group: the logs of its rows' sums, the totals of what the pieces listed, and the k best of them.  A thread fetches
+// eight entries at a time: one workgroup serves a group, so what counts is that no load waits for the one before it.
+constexpr uint32_t JOIN_THREADS = 1024, JOIN_WAVES = JOIN_THREADS / 64, JOIN_AT_ONCE = 8;
+template <int GROUPS, bool NORMALIZE>
+__global__ __launch_bounds__(JOIN_THREADS) void beam_join_kernel(BeamParams p) {
     constexpr uint32_t CAP = 2048;
     __shared__ double s_lse[BEAMS_MAX];
     __shared__ float s_start[BEAMS_MAX];
-    __shared__ uint32_t s_max[256 * GROUPS], s_n, s_cnt[8];
-    __shared__ uint64_t s_ord[CAP], s_entry[CAP];
+    __shared__ uint32_t s_max[256 * GROUPS], s_n, s_bound, s_cnt[2 * JOIN_WAVES];
+    __shared__ __align__(16) uint64_t s_ord[CAP + 8];
+    __shared__ uint64_t s_entry[CAP];
     __shared__ uint16_t s_beam[CAP];
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, group = blockIdx.x;
     const size_t row0 = (size_t)group * p.beams;
-    for (uint32_t b = wave; b < p.beams; b += 4) {
+    for (uint32_t b = wave; b < p.beams; b += JOIN_WAVES) {
         const size_t at = (row0 + b) * p.pieces;
-        const bool ended = p.finished && p.finished[row0 + b];
         double lse = 0.0;
-        if (p.normalize && !ended) {
+        if (NORMALIZE && !(p.finished && p.finished[row0 + b])) {
             float m = -__builtin_inff();
             bool bad = false;
             for (uint32_t i = lane; i < p.pieces; i += 64) {
@@ -255,7 +439,7 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamParams p) {
             bad = __any(bad) || m == __builtin_inff();
             double s = 0.0;
             if (m > -__builtin_inff())
-                for (uint32_t i = lane; i < p.pieces; i += 64) s += p.sum[at + i] * exp_below0((double)p.peak[at + i] - (double)m);
+                for (uint32_t i = lane; i < p.pieces; i += 64) s += p.sum[at + i] * exp64((double)p.peak[at + i] - (double)m);
             s = wave_sum(s);
             lse = bad ? __longlong_as_double(0x7ff8000000000000ll) : (double)m + log(s);
         }
@@ -265,45 +449,49 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamParams p) {
         }
     }
     if (t == 0) s_n = 0;
-#pragma unroll
-    for (int g = 0; g < GROUPS; ++g) s_max[g * 256 + t] = 0;
+    if (t < 256 * GROUPS) s_max[t] = 0;
     __syncthreads();
-    const uint64_t* list = p.list + row0 * p.pieces * p.k;
-    const uint32_t per_row = p.pieces * p.k;
-    const uint64_t slots = (uint64_t)p.beams * per_row;
-    // order of the total, list entry and beam of a slot; an ended beam's entry holds a logit of 0 and no sum
-    auto total_of = [&](uint64_t i, uint64_t* entry, uint32_t* beam) -> uint64_t {
-        const uint64_t e = list[i];
-        if (!e) return 0;
-        const uint32_t b = slots >> 32 ? (uint32_t)(i / per_row) : (uint32_t)i / per_row;
-        *entry = e;
+    const uint64_t* list = p.list + row0 * p.pieces * p.len;
+    const uint32_t slots = p.beams * p.pieces * p.len;  // below 2^31
+    // order of the total and beam of a list entry; an ended beam's entry holds a logit of 0 and no sum
+    auto total_of = [&](uint64_t e, uint32_t i, uint32_t* beam) -> uint64_t {
+        const uint32_t b = (uint32_t)(((uint64_t)i * p.per_row_magic) >> (31 + p.per_row_shift));
         *beam = b;
-        return order64((double)s_start[b] + ((double)ord2f((uint32_t)(e >> 32)) - s_lse[b]));
+        return e ? order64((double)s_start[b] + ((double)ord2f((uint32_t)(e >> 32)) - s_lse[b])) : 0;
     };
-    uint64_t entry = 0;
-    uint32_t beam = 0;
-    {
-        uint32_t m[GROUPS] = {}, g = 0;
-        for (uint64_t i = t; i < slots; i += 256) {
-            const uint32_t h = (uint32_t)(total_of(i, &entry, &beam) >> 32);
+    // f(order, entry, beam, slot) for every slot that holds an entry of a total
+    auto each = [&](auto f) {
+        for (uint32_t i0 = t; i0 < slots; i0 += JOIN_THREADS * JOIN_AT_ONCE) {
+            uint64_t e[JOIN_AT_ONCE];
 #pragma unroll
-            for (uint32_t q = 0; q < GROUPS; ++q)
-                if (q == g) m[q] = max(m[q], h);
-            g = g + 1 == GROUPS ? 0 : g + 1;
+            for (uint32_t u = 0; u < JOIN_AT_ONCE; ++u) e[u] = i0 + u * JOIN_THREADS < slots ? list[i0 + u * JOIN_THREADS] : 0;
+#pragma unroll
+            for (uint32_t u = 0; u < JOIN_AT_ONCE; ++u) {
+                uint32_t beam = 0;
+                const uint64_t o = e[u] ? total_of(e[u], i0 + u * JOIN_THREADS, &beam) : 0;
+                if (o) f(o, e[u], beam, i0 + u * JOIN_THREADS);
+            }
         }
-#pragma unroll
-        for (int q = 0; q < GROUPS; ++q) s_max[q * 256 + t] = m[q];
+    };
+    // Maxima over 256 * GROUPS sets of entries; a piece's entries stand at the front of its list, so the sets are mixed by a
+    // hash of the slot: large totals that shared a set would lower the bound.
+    each([&](uint64_t o, uint64_t, uint32_t, uint32_t i) {
+        atomicMax(&s_max[(i * 2654435761u) >> (GROUPS == 1 ? 24 : 22)], (uint32_t)(o >> 32));
+    });
+    __syncthreads();
+    if (wave == 0) {
+        const uint32_t kth = kth_largest<4 * GROUPS>(s_max, p.k, lane);
+        if (lane == 0) s_bound = kth;
     }
     __syncthreads();
-    const uint32_t pivot = kth_largest<4 * GROUPS>(s_max, p.k, lane);
-    auto keep = [&](uint64_t o) {
+    const uint32_t bound = s_bound;
+    auto keep = [&](uint64_t o, uint64_t e, uint32_t beam) {
         const uint32_t at = atomicAdd(&s_n, 1u);
-        if (at < CAP) { s_ord[at] = o; s_entry[at] = entry; s_beam[at] = (uint16_t)beam; }
+        if (at < CAP) { s_ord[at] = o; s_entry[at] = e; s_beam[at] = (uint16_t)beam; }
     };
-    for (uint64_t i = t; i < slots; i += 256) {
-        const uint64_t o = total_of(i, &entry, &beam);
-        if (o && (uint32_t)(o >> 32) >= pivot) keep(o);
-    }
+    each([&](uint64_t o, uint64_t e, uint32_t beam, uint32_t) {
+        if ((uint32_t)(o >> 32) >= bound) keep(o, e, beam);
+    });
     __syncthreads();
     uint32_t n = s_n;
     if (n > CAP) {
@@ -314,53 +502,66 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamParams p) {
         for (int bit = 63; bit >= 0; --bit) {
             const uint64_t cand = kth | (1ull << bit);
             c = 0;
-            for (uint64_t i = t; i < slots; i += 256) c += total_of(i, &entry, &beam) >= cand;
-            if (block_count(c, s_cnt, turn++) >= p.k) kth = cand;
+            each([&](uint64_t o, uint64_t, uint32_t, uint32_t) { c += o >= cand; });
+            if (block_count<JOIN_WAVES>(c, s_cnt, turn++) >= p.k) kth = cand;
         }
         c = 0;
-        for (uint64_t i = t; i < slots; i += 256) c += total_of(i, &entry, &beam) > kth;
-        uint32_t need = p.k - block_count(c, s_cnt, turn++);
+        each([&](uint64_t o, uint64_t, uint32_t, uint32_t) { c += o > kth; });
+        uint32_t need = p.k - block_count<JOIN_WAVES>(c, s_cnt, turn++);
         for (int bit = 9; bit >= 0; --bit) {  // the largest beam that fewer than `need` of the equal ones lie before
             const uint32_t cand = last_beam | (1u << bit);
             c = 0;
-            for (uint64_t i = t; i < slots; i += 256) c += total_of(i, &entry, &beam) == kth && beam < cand;
-            if (block_count(c, s_cnt, turn++) < need) last_beam = cand;
+            each([&](uint64_t o, uint64_t, uint32_t b, uint32_t) { c += o == kth && b < cand; });
+            if (block_count<JOIN_WAVES>(c, s_cnt, turn++) < need) last_beam = cand;
         }
         c = 0;
-        for (uint64_t i = t; i < slots; i += 256) c += total_of(i, &entry, &beam) == kth && beam < last_beam;
-        need -= block_count(c, s_cnt, turn++);
+        each([&](uint64_t o, uint64_t, uint32_t b, uint32_t) { c += o == kth && b < last_beam; });
+        need -= block_count<JOIN_WAVES>(c, s_cnt, turn++);
         for (int bit = 63; bit >= 0; --bit) {  // entries count down: ~entry ascends
             const uint64_t cand = last | (1ull << bit);
             c = 0;
-            for (uint64_t i = t; i < slots; i += 256) c += total_of(i, &entry, &beam) == kth && beam == last_beam && ~entry < cand;
-            if (block_count(c, s_cnt, turn++) < need) last = cand;
+            each([&](uint64_t o, uint64_t e, uint32_t b, uint32_t) { c += o == kth && b == last_beam && ~e < cand; });
+            if (block_count<JOIN_WAVES>(c, s_cnt, turn++) < need) last = cand;
         }
         __syncthreads();
         if (t == 0) s_n = 0;
         __syncthreads();
-        for (uint64_t i = t; i < slots; i += 256) {
-            const uint64_t o = total_of(i, &entry, &beam);
-            if (o > kth || (o == kth && (beam < last_beam || (beam == last_beam && ~entry <= last)))) keep(o);
-        }
+        each([&](uint64_t o, uint64_t e, uint32_t b, uint32_t) {
+            if (o > kth || (o == kth && (b < last_beam || (b == last_beam && ~e <= last)))) keep(o, e, b);
+        });
         __syncthreads();
         n = s_n;  // k
     }
     uint32_t* parents = p.out_parents + (size_t)group * p.k;
     uint32_t* tokens = p.out_tokens + (size_t)group * p.k;
     float* scores = p.out_scores + (size_t)group * p.k;
-    for (uint32_t i = t; i < n; i += 256) {
+    if (t < 8) s_ord[n + t] = 0;
+    __syncthreads();
+    for (uint32_t i = t; i < n; i += JOIN_THREADS) {
         const uint64_t o = s_ord[i], e = s_entry[i];
         const uint32_t b = s_beam[i];
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; ++j)
-            rank += s_ord[j] > o || (s_ord[j] == o && (s_beam[j] < b || (s_beam[j] == b && s_entry[j] > e)));
+        for (uint32_t j = 0; j < n; j += 8) {
+            uint64_t other[8];
+            bool same = false;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) other[u] = s_ord[j + u];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                rank += other[u] > o;
+                same |= other[u] == o && j + u != i;
+            }
+            if (same)  // equal totals: by beam, then by logit and token
+                for (uint32_t u = j; u < min(j + 8, n); ++u)
+                    rank += s_ord[u] == o && (s_beam[u] < b || (s_beam[u] == b && s_entry[u] > e));
+        }
         if (rank < p.k) {
             parents[rank] = b;
             tokens[rank] = (uint32_t)~(uint32_t)e;
             scores[rank] = (float)of_order64(o);
         }
     }
-    for (uint32_t i = n + t; i < p.k; i += 256) {
+    for (uint32_t i = n + t; i < p.k; i += JOIN_THREADS) {
         parents[i] = tokens[i] = 0xffffffffu;
         scores[i] = -__builtin_inff();
     }
@@ -431,13 +632,31 @@ static hipError_t launch_moves(const uint32_t* d_parents, uint32_t groups, uint3
 }
 
 // ---- host side ---------------------------------------------------------------------------------
-template <typename V>
-static void launch_pieces(const BeamParams& p, hipStream_t stream) {
-    const dim3 grid(p.rows * p.pieces);
-    if (p.k <= 64) hipLaunchKernelGGL((beam_piece_kernel<V, 32, 1>), grid, dim3(PIECE_THREADS), 0, stream, p);
-    else hipLaunchKernelGGL((beam_piece_kernel<V, 32, 4>), grid, dim3(PIECE_THREADS), 0, stream, p);
+// Bytes of a row per thread and chunk.  64 x 8 rows of 131072 bf16 logits: 59 us with 32 (114 registers, four workgroups
+// per CU), 80 us with 64 (164 registers, three).
+constexpr uint32_t LONG_BYTES = 32;
+// Workgroups per CU that the pieces are cut for: the same rows take 59 us with 4, 72 us with 5, 70 us with 8, 78 us with 16.
+constexpr uint32_t PIECES_PER_CU = 4;
+template <typename V, int EACH, int GROUPS>
+static void launch_pieces_of(const BeamParams& p, bool normalize, hipStream_t stream) {
+    const dim3 grid(p.rows * p.pieces), block(PIECE_THREADS);
+    if (normalize && p.mask) hipLaunchKernelGGL((beam_piece_kernel<V, EACH, GROUPS, true, true>), grid, block, 0, stream, p);
+    else if (normalize) hipLaunchKernelGGL((beam_piece_kernel<V, EACH, GROUPS, true, false>), grid, block, 0, stream, p);
+    else if (p.mask) hipLaunchKernelGGL((beam_piece_kernel<V, EACH, GROUPS, false, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((beam_piece_kernel<V, EACH, GROUPS, false, false>), grid, block, 0, stream, p);
 }
-constexpr uint32_t PIECE_LEN = PIECE_THREADS * 32;
+template <typename V>
+static void launch_pieces(const BeamParams& p, bool normalize, bool short_chunks, hipStream_t stream) {
+    // 256 maxima tell the k <= 64 largest of a chunk well enough (about 1.2 k logits reach the bound), more need 1024
+    if (short_chunks) {
+        if (p.k <= 64) launch_pieces_of<V, 8, 1>(p, normalize, stream);
+        else launch_pieces_of<V, 8, 4>(p, normalize, stream);
+    } else if (p.k <= 64) {
+        launch_pieces_of<V, (int)LONG_BYTES / V::size, 1>(p, normalize, stream);
+    } else {
+        launch_pieces_of<V, (int)LONG_BYTES / V::size, 4>(p, normalize, stream);
+    }
+}
 
 static needle_hip_status states_check(const needle_beam_state* states, uint32_t n_states, uint64_t rows, uint64_t picks) {
     if (n_states && !states) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "states is null");
@@ -530,17 +749,36 @@ static needle_hip_status select_enqueue(needle_hip_ctx* c, const needle_beam_par
         HIP_TRY(hipGetLastError());
         return NEEDLE_HIP_OK;
     }
+    const bool normalize = q.normalize != 0;
     BeamParams p{};
-    p.beams = q.beams; p.vocab = q.vocab; p.k = q.k; p.end_token = q.end_token; p.normalize = q.normalize != 0;
+    p.beams = q.beams; p.vocab = q.vocab; p.k = q.k; p.end_token = q.end_token;
     p.row_stride = q.row_stride; p.mask_stride = q.mask_stride;
-    p.pieces = (q.vocab + PIECE_LEN - 1) / PIECE_LEN;
+    // Few rows: chunks of 2048 logits, a workgroup each, so that more of the chip works on a row.  Otherwise chunks of
+    // LONG_BYTES per thread, and as many pieces as give the chip about PIECES_PER_CU workgroups per CU.
+    const uint64_t all_rows = (uint64_t)q.groups * q.beams;
+    const uint64_t long_chunk = PIECE_THREADS * LONG_BYTES / value_size(q.value), long_chunks = (q.vocab + long_chunk - 1) / long_chunk;
+    const bool short_chunks = all_rows * long_chunks < 2ull * c->n_cu;
+    if (short_chunks) {
+        p.chunks_per_piece = 1;
+        p.pieces = (q.vocab + 2047) / 2048;
+    } else {
+        const uint64_t want = std::min<uint64_t>(long_chunks, std::max<uint64_t>(1, ((uint64_t)PIECES_PER_CU * c->n_cu + all_rows - 1) / all_rows));
+        p.chunks_per_piece = (uint32_t)((long_chunks + want - 1) / want);
+        p.pieces = (uint32_t)((long_chunks + p.chunks_per_piece - 1) / p.chunks_per_piece);
+    }
+    p.len = std::max<uint32_t>(2 * q.k, 32);  // room for what the last bound lets through, so that few lists need an exact cut
+    {
+        const uint32_t d = p.pieces * p.len;  // rounded up 32-bit reciprocal: exact for numerators below 2^31
+        while ((1ull << p.per_row_shift) < d) ++p.per_row_shift;
+        p.per_row_magic = (uint32_t)((((1ull << 31) << p.per_row_shift) + d - 1) / d);
+    }
     // a block of groups at a time: the pieces' lists stay within 256 MiB (one group's may be more), the grid within 2^22
-    const uint64_t group_pieces = (uint64_t)q.beams * p.pieces, piece_bytes = (uint64_t)q.k * 8 + 12;
+    const uint64_t group_pieces = (uint64_t)q.beams * p.pieces, piece_bytes = (uint64_t)p.len * 8 + 12;
     uint64_t blk = std::min<uint64_t>((256ull << 20) / (group_pieces * piece_bytes), (1u << 22) / group_pieces);
     blk = std::max<uint64_t>(1, std::min<uint64_t>(blk, q.groups));
     HIP_TRY(c->scratch[7].ensure(blk * group_pieces * piece_bytes));
     p.list = c->scratch[7].as<uint64_t>();
-    p.sum = (double*)(p.list + blk * group_pieces * q.k);
+    p.sum = (double*)(p.list + blk * group_pieces * p.len);
     p.peak = (float*)(p.sum + blk * group_pieces);
     for (uint64_t g0 = 0; g0 < q.groups; g0 += blk) {
         const uint64_t r0 = g0 * q.beams;
@@ -552,13 +790,16 @@ static needle_hip_status select_enqueue(needle_hip_ctx* c, const needle_beam_par
         p.mask = q.mask ? q.mask + r0 * q.mask_stride : nullptr;
         p.out_parents = parents + g0 * q.k; p.out_tokens = tokens + g0 * q.k; p.out_scores = scores + g0 * q.k; p.out_counts = counts + g0;
         switch (q.value) {
-        case NEEDLE_VALUE_F32: launch_pieces<ValueF32>(p, c->stream); break;
-        case NEEDLE_VALUE_F16: launch_pieces<ValueF16>(p, c->stream); break;
-        default: launch_pieces<ValueBF16>(p, c->stream);
+        case NEEDLE_VALUE_F32: launch_pieces<ValueF32>(p, normalize, short_chunks, c->stream); break;
+        case NEEDLE_VALUE_F16: launch_pieces<ValueF16>(p, normalize, short_chunks, c->stream); break;
+        default: launch_pieces<ValueBF16>(p, normalize, short_chunks, c->stream);
         }
         HIP_TRY(hipGetLastError());
-        if (q.k <= 64) hipLaunchKernelGGL((beam_join_kernel<1>), dim3(p.groups), dim3(256), 0, c->stream, p);
-        else hipLaunchKernelGGL((beam_join_kernel<4>), dim3(p.groups), dim3(256), 0, c->stream, p);
+        const dim3 grid(p.groups), block(JOIN_THREADS);
+        if (q.k <= 64 && normalize) hipLaunchKernelGGL((beam_join_kernel<1, true>), grid, block, 0, c->stream, p);
+        else if (q.k <= 64) hipLaunchKernelGGL((beam_join_kernel<1, false>), grid, block, 0, c->stream, p);
+        else if (normalize) hipLaunchKernelGGL((beam_join_kernel<4, true>), grid, block, 0, c->stream, p);
+        else hipLaunchKernelGGL((beam_join_kernel<4, false>), grid, block, 0, c->stream, p);
         HIP_TRY(hipGetLastError());
     }
     return NEEDLE_HIP_OK;
