@@ -87,67 +87,398 @@ struct MatmulParams {
     uint32_t m, k;
 };
 
-// 16 codes of a row from place `at` on, zero from k on; nothing outside the row is read.
+// 16 codes of a row from place `at` on, zero from k on; nothing outside the row is read.  The last codes of a row are the
+// end of the 16 that end with it, shifted down.
 __device__ inline u32x4 load_codes(const int8_t* row, uint32_t at, uint32_t k) {
     if (at + 16 <= k) return *(const u32x4_any*)(row + at);
+    if (at >= k) return u32x4{0, 0, 0, 0};
+    if (k >= 16) {
+        const u32x4 v = *(const u32x4_any*)(row + k - 16);
+        const uint64_t lo = v[0] | (uint64_t)v[1] << 32, hi = v[2] | (uint64_t)v[3] << 32;
+        const uint32_t bits = (at + 16 - k) * 8;  // 8 .. 120
+        const uint64_t a = bits < 64 ? lo >> bits | hi << (64 - bits) : hi >> (bits - 64), b = bits < 64 ? hi >> bits : 0;
+        return u32x4{(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)};
+    }
     uint32_t w[4] = {0, 0, 0, 0};
     for (uint32_t j = 0; at + j < k; ++j) w[j >> 2] |= (uint32_t)(uint8_t)row[at + j] << (8 * (j & 3));
     return u32x4{w[0], w[1], w[2], w[3]};
 }
 
-// Any sizes, strides and alignment.  A workgroup makes 64 rows of b x 64 rows of a: both pass through LDS in slices of
-// 64 codes (rows of 80 bytes: the 16-byte reads of a quarter wave meet every bank once).  The rows of b are the matrix
-// instruction's rows, so a lane ends up with four neighbouring outputs of one row of `out`.
-template <typename V>
-__global__ __launch_bounds__(256) void matmul_i8_kernel(MatmulParams p) {
-    __shared__ __align__(16) uint8_t s_b[64][80], s_a[64][80];
-    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, l15 = lane & 15, quad = lane >> 4;
-    const uint64_t tiles_n = (p.n + 63) / 64, tiles = tiles_n * ((p.m + 63) / 64);
-    for (uint64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const uint64_t n0 = tile % tiles_n * 64;
-        const uint32_t m0 = (uint32_t)(tile / tiles_n) * 64;
-        const uint32_t r = t >> 2, ch = (t & 3) * 16;
-        const int8_t* rb = p.b + min(n0 + r, p.n - 1) * p.b_stride;  // rows behind the last: a copy of it, never stored
-        const int8_t* ra = p.a + (uint64_t)min(m0 + r, p.m - 1) * p.a_stride;
-        i32x4 acc[4] = {};
-        for (uint32_t k0 = 0; k0 < p.k; k0 += 64) {
-            const u32x4 vb = load_codes(rb, k0 + ch, p.k), va = load_codes(ra, k0 + ch, p.k);
-            __syncthreads();
-            *(u32x4*)&s_b[r][ch] = vb;
-            *(u32x4*)&s_a[r][ch] = va;
-            __syncthreads();
-            const i32x4 fb = *(const i32x4*)&s_b[wave * 16 + l15][quad * 16];
+// Four neighbouring values of a column vector from j on; behind the last of n the last one again.
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+__device__ inline f32x4_any four_of(const float* v, uint64_t j, uint64_t n) {
+    if (j + 4 <= n) return *(const f32x4_any*)(v + j);
+    f32x4_any y;
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                acc[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb, *(const i32x4*)&s_a[q * 16 + l15][quad * 16], acc[q], 0, 0, 0);
+    for (int e = 0; e < 4; ++e) y[e] = v[min(j + e, n - 1)];
+    return y;
+}
+// Four neighbouring outputs of a row from j on, as far as there are any.  Everything is in registers: a load in here would
+// wait for the stores before it.
+template <typename V>
+__device__ inline void store_four(typename V::bits* row, uint64_t j, uint64_t n, i32x4 sums, float sa, f32x4_any sb, bool biased, f32x4_any bias) {
+    typedef typename V::bits four_t __attribute__((ext_vector_type(4), aligned(V::size)));
+    four_t v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float y = (float)sums[e] * sa * sb[e];
+        if (biased) y += bias[e];
+        v[e] = V::round(y);
+    }
+    if (j + 4 <= n) {
+        *(four_t*)(row + j) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if (j + e < n) row[j + e] = v[e];
+    }
+}
+
+// ---- few rows of a ---------------------------------------------------------------------------
+// At most 16 * NA rows of a: what counts is the stream over b.  A wave takes 16 * NB rows of b straight from memory into the
+// matrix instruction's registers (16 bytes per lane, 64 codes of a row per load), those of a from the cache, the next slice
+// under way while one is multiplied.  SPLIT: the four waves of a workgroup share the rows and take every fourth slice, so
+// that a short table still has the whole chip at work; their sums meet in LDS (whole numbers: any order is exact).
+template <typename V, int NB, int NA, bool SPLIT>
+__global__ __launch_bounds__(256) void matmul_i8_stream_kernel(MatmulParams p) {
+    constexpr uint32_t STEP = SPLIT ? 4 : 1;
+    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, l15 = lane & 15, quad = lane >> 4;
+    const uint64_t n0 = (SPLIT ? (uint64_t)blockIdx.x : (uint64_t)blockIdx.x * 4 + wave) * (16 * NB);
+    if (!SPLIT && n0 >= p.n) return;
+    const int8_t* rb[NB];
+    const int8_t* ra[NA];
+#pragma unroll
+    for (int x = 0; x < NB; ++x) rb[x] = p.b + min(n0 + x * 16 + l15, p.n - 1) * p.b_stride + quad * 16;
+#pragma unroll
+    for (int y = 0; y < NA; ++y) ra[y] = p.a + (uint64_t)min(y * 16 + l15, p.m - 1) * p.a_stride + quad * 16;
+    i32x4 acc[NB][NA] = {};
+    u32x4 fb[2][NB], fa[2][NA];
+    auto load = [&](uint32_t s, u32x4 (&b)[NB], u32x4 (&a)[NA]) {
+        const uint32_t at = s * 64;
+        if (at + 64 <= p.k) {
+#pragma unroll
+            for (int x = 0; x < NB; ++x) b[x] = *(const u32x4_any*)(rb[x] + at);
+#pragma unroll
+            for (int y = 0; y < NA; ++y) a[y] = *(const u32x4_any*)(ra[y] + at);
+        } else {
+#pragma unroll
+            for (int x = 0; x < NB; ++x) b[x] = load_codes(rb[x] - quad * 16, at + quad * 16, p.k);
+#pragma unroll
+            for (int y = 0; y < NA; ++y) a[y] = load_codes(ra[y] - quad * 16, at + quad * 16, p.k);
+        }
+    };
+    auto multiply = [&](const u32x4 (&b)[NB], const u32x4 (&a)[NA]) {
+#pragma unroll
+        for (int x = 0; x < NB; ++x)
+#pragma unroll
+            for (int y = 0; y < NA; ++y)
+                acc[x][y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, b[x]), __builtin_bit_cast(i32x4, a[y]), acc[x][y], 0, 0, 0);
+    };
+    const uint32_t slices = (p.k + 63) / 64;
+    uint32_t s = SPLIT ? wave : 0;
+    if (s < slices) load(s, fb[0], fa[0]);
+    for (; s < slices; s += 2 * STEP) {
+        if (s + STEP < slices) load(s + STEP, fb[1], fa[1]);
+        multiply(fb[0], fa[0]);
+        if (s + STEP >= slices) break;
+        if (s + 2 * STEP < slices) load(s + 2 * STEP, fb[0], fa[0]);
+        multiply(fb[1], fa[1]);
+    }
+    const uint64_t j0 = n0 + quad * 4;
+    auto finish = [&](int x) {
+        const uint64_t j = j0 + x * 16;
+        if (j >= p.n) return;
+        const f32x4_any sb = four_of(p.b_scales, j, p.n), bias = p.bias ? four_of(p.bias, j, p.n) : f32x4_any{};
+#pragma unroll
+        for (int y = 0; y < NA; ++y) {
+            const uint32_t i = y * 16 + l15;
+            if (i < p.m) store_four<V>((typename V::bits*)p.out + (uint64_t)i * p.out_stride, j, p.n, acc[x][y], p.a_scales[i], sb, p.bias != nullptr, bias);
+        }
+    };
+    if (SPLIT) {
+        __shared__ i32x4 s_part[4][NB][NA][64];
+#pragma unroll
+        for (int x = 0; x < NB; ++x)
+#pragma unroll
+            for (int y = 0; y < NA; ++y) s_part[wave][x][y][lane] = acc[x][y];
+        __syncthreads();
+        // wave w finishes the w-th share of the tiles of b
+#pragma unroll
+        for (int x = 0; x < NB; ++x) {
+            if ((uint32_t)(NB == 1 ? 0 : x * 4 / NB) != wave) continue;
+#pragma unroll
+            for (int y = 0; y < NA; ++y) acc[x][y] = s_part[0][x][y][lane] + s_part[1][x][y][lane] + s_part[2][x][y][lane] + s_part[3][x][y][lane];
+            finish(x);
+        }
+    } else {
+#pragma unroll
+        for (int x = 0; x < NB; ++x) finish(x);
+    }
+}
+
+// ---- tiles through LDS -----------------------------------------------------------------------
+// A workgroup of WB x WA waves makes TB rows of b x TA rows of a; a wave (TB / WB) x (TA / WA) of them with the 16x16x64
+// instruction.  Slices of 64 codes pass through SLOTS LDS slots; a wave holds the operands of the slice it multiplies in
+// registers and reads those of the next one meanwhile, so that slice s + 1 is read, those behind it are under way, and
+// slot s, which every wave has left, takes slice s + SLOTS -- with one barrier per slice.  A slice's row is four 16-byte chunks,
+// chunk c of row r at place c ^ 2 (r >> 3 & 1): the sixteen 16-byte reads that meet the banks together touch all of them
+// once.  DMA: the loads write LDS themselves (chunks and rows aligned to 16 bytes); otherwise they pass through registers
+// two slices ahead, from any address.
+constexpr uint32_t SLICE = 64;
+__device__ const uint32_t g_zeros[4] = {0, 0, 0, 0};
+typedef __attribute__((address_space(1))) const void glb_cvoid;
+typedef __attribute__((address_space(3))) void lds_void;
+
+template <typename V, int TB, int TA, int WB, int WA, int SLOTS, bool DMA>
+__global__ __launch_bounds__(64 * WB * WA) void matmul_i8_tile_kernel(MatmulParams p, uint32_t tiles_b, uint32_t tiles_a) {
+    constexpr int WAVES = WB * WA, NB = TB / WB / 16, NA = TA / WA / 16, STAGE = (TB + TA) * SLICE, LOADS = (TB + TA) / 16 / WAVES;
+    static_assert((TB + TA) % (16 * WAVES) == 0 && TB % 16 == 0, "every wave fills whole groups of sixteen rows");
+    extern __shared__ __align__(16) uint8_t s_tile[];
+    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, l15 = lane & 15, quad = lane >> 4;
+    const uint32_t wb = wave % WB, wa = wave / WB;
+    // Workgroups go to the chip's eight dies in turn, each with its own L2: a die gets a run of tiles, in groups of four
+    // tiles of a that share their tiles of b.
+    const uint32_t tiles = tiles_b * tiles_a;
+    uint32_t tile;
+    {
+        const uint32_t die = blockIdx.x & 7, nth = blockIdx.x >> 3, each = tiles >> 3, more = tiles & 7;
+        tile = die * each + min(die, more) + nth;
+    }
+    const uint32_t group = 4 * tiles_b, g0 = tile / group * 4, rows = min(4u, tiles_a - g0), in = tile % group;
+    const uint32_t m0 = (g0 + in % rows) * TA;
+    const uint64_t n0 = (uint64_t)(in / rows) * TB;
+
+    // the wave's share of a slice: LOADS times sixteen rows; lane: row lane / 4, place lane % 4
+    const int8_t* from[LOADS];
+    const uint32_t chunk = ((lane & 3) ^ (lane >> 5 << 1)) * 16;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const uint32_t r = (wave + i * WAVES) * 16 + (lane >> 2);
+        from[i] = r < TB ? p.b + min(n0 + r, p.n - 1) * p.b_stride : p.a + (uint64_t)min(m0 + r - TB, p.m - 1) * p.a_stride;
+    }
+    const uint32_t slices = (p.k + SLICE - 1) / SLICE;
+    auto fill = [&](uint32_t s) {
+        uint8_t* to = s_tile + s % SLOTS * STAGE + wave * 1024;
+        const uint32_t at = s * SLICE + chunk;
+        if ((s + 1) * SLICE <= p.k) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i)
+                __builtin_amdgcn_global_load_lds((glb_cvoid*)(from[i] + at), (lds_void*)(to + i * WAVES * 1024), 16, 0, 0);
+            return;
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const uint32_t i = m0 + q * 16 + l15;
-            const uint64_t j0 = n0 + wave * 16 + quad * 4;
-            if (i >= p.m) continue;
-            const float sa = p.a_scales[i];
-            typename V::bits* o = (typename V::bits*)p.out + (uint64_t)i * p.out_stride;
+        for (int i = 0; i < LOADS; ++i)  // chunks behind k are zeros (k is a multiple of 16 here)
+            __builtin_amdgcn_global_load_lds((glb_cvoid*)(at < p.k ? (const void*)(from[i] + at) : (const void*)g_zeros),
+                                             (lds_void*)(to + i * WAVES * 1024), 16, 0, 0);
+    };
+    auto fetch = [&](uint32_t s, u32x4 (&held)[LOADS]) {
+        const uint32_t at = s * SLICE;
+        if (at + SLICE <= p.k) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (j0 + e >= p.n) break;
-                float y = (float)acc[q][e] * sa * p.b_scales[j0 + e];
-                if (p.bias) y += p.bias[j0 + e];
-                o[j0 + e] = V::round(y);
+            for (int i = 0; i < LOADS; ++i) held[i] = *(const u32x4_any*)(from[i] + at + chunk);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) held[i] = load_codes(from[i], at + chunk, p.k);
+        }
+    };
+    auto store = [&](uint32_t s, const u32x4 (&held)[LOADS]) {
+        uint8_t* to = s_tile + s % SLOTS * STAGE + wave * 1024 + lane * 16;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) *(u32x4*)(to + i * WAVES * 1024) = held[i];
+    };
+    const uint32_t place = (quad ^ (l15 >> 3 << 1)) * 16;
+    const uint32_t off_b = (wb * (TB / WB) + l15) * SLICE + place, off_a = (TB + wa * (TA / WA) + l15) * SLICE + place;
+    i32x4 acc[NB][NA] = {};
+    i32x4 fb[2][NB], fa[2][NA];
+    auto read = [&](uint32_t s, i32x4 (&b)[NB], i32x4 (&a)[NA]) {
+        const uint8_t* buf = s_tile + s % SLOTS * STAGE;
+#pragma unroll
+        for (int x = 0; x < NA; ++x) a[x] = *(const i32x4*)(buf + off_a + x * 16 * SLICE);
+#pragma unroll
+        for (int x = 0; x < NB; ++x) b[x] = *(const i32x4*)(buf + off_b + x * 16 * SLICE);
+    };
+    auto multiply = [&](const i32x4 (&b)[NB], const i32x4 (&a)[NA]) {
+#pragma unroll
+        for (int x = 0; x < NB; ++x)
+#pragma unroll
+            for (int y = 0; y < NA; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[x], a[y], acc[x][y], 0, 0, 0);
+    };
+    // The reads are spread among the matrix instructions: issued in a row they would hold them up, one wave's LDS traffic
+    // behind the other waves'.
+    auto spread = [&] {
+#pragma unroll
+        for (int r = 0; r < NB + NA; ++r) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                     // an LDS read
+            __builtin_amdgcn_sched_group_barrier(0x008, NB * NA / (NB + NA), 0);   // matrix instructions
+        }
+    };
+    if (DMA) {
+        // one slice: wait for slice s + 1, leave the barrier, send for slice s + SLOTS, read s + 1, multiply s
+        auto step = [&](uint32_t s, int cur) {
+            if (SLOTS == 4 && s + 3 < slices) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");
+            else if (s + 2 < slices) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave has read slice s out of its slot
+            __builtin_amdgcn_s_barrier();
+            if (s + SLOTS < slices) fill(s + SLOTS);
+            __builtin_amdgcn_sched_barrier(0);
+            read(s + 1, fb[cur ^ 1], fa[cur ^ 1]);  // (behind the last slice: what an earlier one left there, never used)
+            multiply(fb[cur], fa[cur]);
+            spread();
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        for (uint32_t s = 0; s < min(slices, (uint32_t)SLOTS); ++s) fill(s);
+        if (slices) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            read(0, fb[0], fa[0]);
+        }
+        uint32_t s = 0;
+        for (; s + 2 <= slices; s += 2) {
+            step(s, 0);
+            step(s + 1, 1);
+        }
+        if (s < slices) step(s, 0);
+    } else if (slices) {
+        // slot s - 1, which every wave has left, takes the slice fetched two steps ago
+        u32x4 held[2][LOADS];
+        auto step = [&](uint32_t s, int cur) {
+            __syncthreads();
+            if (s + SLOTS - 1 < slices) store(s + SLOTS - 1, held[(cur + SLOTS - 1) & 1]);
+            if (s + SLOTS + 1 < slices) fetch(s + SLOTS + 1, held[(cur + SLOTS - 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            read(s + 1, fb[cur ^ 1], fa[cur ^ 1]);
+            multiply(fb[cur], fa[cur]);
+            spread();
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        for (uint32_t s = 0; s < min(slices, SLOTS - 1u); ++s) {
+            fetch(s, held[0]);
+            store(s, held[0]);
+        }
+        if (SLOTS - 1 < slices) fetch(SLOTS - 1, held[(SLOTS - 1) & 1]);
+        if (SLOTS < slices) fetch(SLOTS, held[SLOTS & 1]);
+        __syncthreads();
+        read(0, fb[0], fa[0]);
+        uint32_t s = 0;
+        for (; s + 2 <= slices; s += 2) {
+            step(s, 0);
+            step(s + 1, 1);
+        }
+        if (s < slices) step(s, 0);
+    }
+    const uint64_t j0 = n0 + wb * (TB / WB) + quad * 4;
+    const uint32_t i0 = m0 + wa * (TA / WA) + l15;
+    f32x4_any sb[NB], bias[NB];
+    float sa[NA];
+#pragma unroll
+    for (int x = 0; x < NB; ++x) {
+        sb[x] = four_of(p.b_scales, j0 + x * 16, p.n);
+        bias[x] = p.bias ? four_of(p.bias, j0 + x * 16, p.n) : f32x4_any{-0.0f, -0.0f, -0.0f, -0.0f};  // x + -0 is x
+    }
+#pragma unroll
+    for (int y = 0; y < NA; ++y) sa[y] = p.a_scales[min(i0 + y * 16, p.m - 1)];
+    typedef typename V::bits four_t __attribute__((ext_vector_type(4), aligned(V::size)));
+    auto four = [&](int x, int y) {
+        four_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = V::round((float)acc[x][y][e] * sa[y] * sb[x][e] + bias[x][e]);
+        return v;
+    };
+    typename V::bits* o = (typename V::bits*)p.out + (uint64_t)i0 * p.out_stride + j0;
+    if (n0 + TB <= p.n && m0 + TA <= p.m) {
+        // Through the wave's own part of LDS, so that a store writes whole lines: 16 bytes per lane along a row instead of
+        // four outputs here and there.  16-byte chunk c of row r lies at place c ^ r (mod the row's chunks).
+        constexpr int LINE = TB / WB * V::size, CHUNKS = LINE / 16, GO = 64 / CHUNKS;  // bytes and chunks of a row; rows per store
+        constexpr int PASS = V::size == 4 ? 1 : NA, ROWS = PASS * 16;  // f32: sixteen rows at a time
+        static_assert(ROWS * LINE * WAVES <= SLOTS * STAGE && CHUNKS <= 64 && ROWS % GO == 0, "the waves' parts fit");
+        uint8_t* part = s_tile + wave * (ROWS * LINE);
+        __syncthreads();
+        o = (typename V::bits*)p.out + (uint64_t)(m0 + wa * (TA / WA)) * p.out_stride + n0 + wb * (TB / WB);
+#pragma unroll
+        for (int y0 = 0; y0 < NA; y0 += PASS) {
+#pragma unroll
+            for (int y = 0; y < PASS; ++y)
+#pragma unroll
+                for (int x = 0; x < NB; ++x) {
+                    const uint32_t r = y * 16 + l15, byte = (x * 16 + quad * 4) * V::size;
+                    *(four_t*)__builtin_assume_aligned(part + r * LINE + (((byte >> 4) ^ r) & (CHUNKS - 1)) * 16 + (byte & 15), 4 * V::size) = four(x, y0 + y);
+                }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int g = 0; g < ROWS / GO; ++g) {
+                const uint32_t r = g * GO + lane / CHUNKS, c = lane % CHUNKS;
+                const u32x4 v = *(const u32x4*)(part + r * LINE + ((c ^ r) & (CHUNKS - 1)) * 16);
+                *(u32x4_any*)((uint8_t*)(o + (uint64_t)(y0 * 16 + r) * p.out_stride) + c * 16) = v;
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    } else {
+#pragma unroll
+        for (int y = 0; y < NA; ++y) {
+            if (i0 + y * 16 >= p.m) continue;
+#pragma unroll
+            for (int x = 0; x < NB; ++x) {
+                const four_t v = four(x, y);
+                typename V::bits* at = o + (uint64_t)(y * 16) * p.out_stride + x * 16;
+                if (j0 + x * 16 + 4 <= p.n) {
+                    *(four_t*)at = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        if (j0 + x * 16 + e < p.n) at[e] = v[e];
+                }
             }
         }
     }
 }
 
-static hipError_t launch_matmul_i8(const MatmulParams& p, int out_value, hipStream_t stream) {
-    const uint64_t tiles = ((p.n + 63) / 64) * ((p.m + 63) / 64);
-    const dim3 grid((uint32_t)std::min<uint64_t>(tiles, 1u << 22));
-    switch (out_value) {
-    case NEEDLE_VALUE_F32: hipLaunchKernelGGL((matmul_i8_kernel<ValueF32>), grid, dim3(256), 0, stream, p); break;
-    case NEEDLE_VALUE_F16: hipLaunchKernelGGL((matmul_i8_kernel<ValueF16>), grid, dim3(256), 0, stream, p); break;
-    default: hipLaunchKernelGGL((matmul_i8_kernel<ValueBF16>), grid, dim3(256), 0, stream, p);
-    }
+template <typename V, int TB, int TA, int WB, int WA, int SLOTS, bool DMA>
+static hipError_t launch_tiles_of(const MatmulParams& p, hipStream_t stream) {
+    constexpr uint32_t lds = SLOTS * (TB + TA) * SLICE;
+    static const hipError_t allowed =
+        hipFuncSetAttribute((const void*)matmul_i8_tile_kernel<V, TB, TA, WB, WA, SLOTS, DMA>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (allowed != hipSuccess) return allowed;
+    const uint32_t tiles_b = (uint32_t)((p.n + TB - 1) / TB), tiles_a = (p.m + TA - 1) / TA;
+    hipLaunchKernelGGL((matmul_i8_tile_kernel<V, TB, TA, WB, WA, SLOTS, DMA>), dim3(tiles_b * tiles_a), dim3(64 * WB * WA), lds, stream, p, tiles_b, tiles_a);
     return hipGetLastError();
+}
+template <typename V, int NB, int NA, bool SPLIT>
+static hipError_t launch_stream_of(const MatmulParams& p, hipStream_t stream) {
+    const uint64_t tiles = (p.n + 16 * NB - 1) / (16 * NB);
+    hipLaunchKernelGGL((matmul_i8_stream_kernel<V, NB, NA, SPLIT>), dim3((uint32_t)(SPLIT ? tiles : (tiles + 3) / 4)), dim3(256), 0, stream, p);
+    return hipGetLastError();
+}
+template <typename V>
+static hipError_t launch_matmul_of(const MatmulParams& p, int n_cu, hipStream_t stream) {
+    const bool aligned = p.k % 16 == 0 && p.a_stride % 16 == 0 && p.b_stride % 16 == 0 && (uintptr_t)p.a % 16 == 0 && (uintptr_t)p.b % 16 == 0;
+    if (p.m <= 16) {
+        // split: long rows of a short table.  Otherwise many short-lived waves of one tile each hide the latency best.
+        const bool split = p.n < 256ull * n_cu && p.k > 256;
+        if (!split) return launch_stream_of<V, 1, 1, false>(p, stream);
+        return p.n < 64ull * n_cu ? launch_stream_of<V, 2, 1, true>(p, stream) : launch_stream_of<V, 4, 1, true>(p, stream);
+    }
+    // Tiles, by what fills the chip (us of the kernel, sizes m x n x k).  A long product of many 256 x 256 tiles is bound by the
+    // matrix cores and the power they draw: 8192 x 8192 x 4096 takes 247 with them, 480 with 128 x 128.  Shorter or fewer:
+    // 128 x 128 (2048 x 2048 x 2048: 21, against 24 with 128 x 64 and 38 with 256 x 256; 1000 x 100000 x 128, bound by its
+    // output: 98, against 110 with 256 x 256); below half a tile per CU 128 x 64 and 64 x 64 (512 x 512 x 4096: 18 with
+    // 64 x 64, 25 with 128 x 128).
+    const auto tiles = [&](uint64_t tb, uint64_t ta) { return ((p.n + tb - 1) / tb) * ((p.m + ta - 1) / ta); };
+    const uint64_t cu = (uint64_t)n_cu;
+    if (p.m > 128 && tiles(256, 256) >= cu && p.k >= 512)
+        return aligned ? launch_tiles_of<V, 256, 256, 2, 4, 4, true>(p, stream) : launch_tiles_of<V, 256, 128, 4, 2, 4, false>(p, stream);
+    if (p.m > 64 && tiles(128, 128) >= cu / 2)
+        return aligned ? launch_tiles_of<V, 128, 128, 4, 2, 4, true>(p, stream) : launch_tiles_of<V, 128, 128, 4, 2, 4, false>(p, stream);
+    if (tiles(128, 64) >= cu)
+        return aligned ? launch_tiles_of<V, 128, 64, 2, 2, 4, true>(p, stream) : launch_tiles_of<V, 128, 64, 2, 2, 4, false>(p, stream);
+    return aligned ? launch_tiles_of<V, 64, 64, 2, 2, 4, true>(p, stream) : launch_tiles_of<V, 64, 64, 2, 2, 4, false>(p, stream);
+}
+static hipError_t launch_matmul_i8(const MatmulParams& p, int out_value, int n_cu, hipStream_t stream) {
+    switch (out_value) {
+    case NEEDLE_VALUE_F32: return launch_matmul_of<ValueF32>(p, n_cu, stream);
+    case NEEDLE_VALUE_F16: return launch_matmul_of<ValueF16>(p, n_cu, stream);
+    default: return launch_matmul_of<ValueBF16>(p, n_cu, stream);
+    }
 }
 
 constexpr uint32_t I8_K_MAX = 131071;  // 2^14 per product at most, sums below 2^31
@@ -248,7 +579,7 @@ extern "C" needle_hip_status needle_hip_matmul_i8_device(needle_hip_ctx* c, cons
     DeviceScope dev(c->device);
     HIP_TRY(dev.error());
     const MatmulParams p{d_a, d_b, d_a_scales, d_b_scales, d_bias, d_out, a_stride, b_stride, out_stride, n, m, k};
-    HIP_TRY(launch_matmul_i8(p, out_value, c->stream));
+    HIP_TRY(launch_matmul_i8(p, out_value, c->n_cu, c->stream));
     HIP_TRY(hipStreamSynchronize(c->stream));
     return NEEDLE_HIP_OK;
 }
@@ -270,7 +601,7 @@ extern "C" needle_hip_status needle_hip_matmul_i8(needle_hip_ctx* c, const int8_
         if (sizes[i]) HIP_TRY(hipMemcpyAsync(d + at[i], src[i], sizes[i], hipMemcpyHostToDevice, c->stream));
     const MatmulParams p{(const int8_t*)(d + at[0]), (const int8_t*)(d + at[1]), (const float*)(d + at[2]), (const float*)(d + at[3]),
                          bias ? (const float*)(d + at[4]) : nullptr, d + at[5], k, k, n, n, m, k};
-    HIP_TRY(launch_matmul_i8(p, NEEDLE_VALUE_F32, c->stream));
+    HIP_TRY(launch_matmul_i8(p, NEEDLE_VALUE_F32, c->n_cu, c->stream));
     HIP_TRY(hipMemcpyAsync(out, d + at[5], sizes[5], hipMemcpyDeviceToHost, c->stream));
     HIP_TRY(hipStreamSynchronize(c->stream));
     return NEEDLE_HIP_OK;
@@ -292,7 +623,7 @@ extern "C" needle_hip_status needle_hip_linear_i8_device(needle_hip_ctx* c, cons
     float* d_scales = (float*)(d_codes + (size_t)m * stride);
     HIP_TRY(launch_quantize_rows(d_x, x_value, m, k, x_stride, d_codes, stride, d_scales, c->stream));
     const MatmulParams p{d_codes, d_b, d_scales, d_b_scales, d_bias, d_out, stride, b_stride, out_stride, n, m, k};
-    HIP_TRY(launch_matmul_i8(p, out_value, c->stream));
+    HIP_TRY(launch_matmul_i8(p, out_value, c->n_cu, c->stream));
     HIP_TRY(hipStreamSynchronize(c->stream));
     return NEEDLE_HIP_OK;
 }

@@ -155,7 +155,8 @@ def _check_product(out, a, sa, b, sb, bias, dtype):
 
 SHAPES = [(1, 1, 1), (1, 17, 16), (3, 5, 7), (16, 16, 64), (17, 33, 65), (1, 1000, 128), (4, 130, 1024), (5, 2049, 384), (64, 64, 63), (65, 127, 300),
           (128, 128, 128), (130, 257, 256), (200, 700, 80), (256, 256, 512), (257, 513, 1008), (300, 1000, 1000), (1, 300, 4096), (16, 515, 5000),
-          (33, 64, 2048), (512, 768, 272), (70, 40, 16), (1000, 3, 96), (2, 9, 9999)]
+          (33, 64, 2048), (512, 768, 272), (70, 40, 16), (1000, 3, 96), (2, 9, 9999), (4112, 4097, 528), (4100, 4105, 513), (1500, 1700, 192), (1500, 1701, 67), (50, 33_000, 96),
+          (20, 20_000, 33), (16, 17_000, 400), (7, 20_000, 700)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
