@@ -424,35 +424,44 @@ __global__ __launch_bounds__(JOIN_THREADS) void beam_join_kernel(BeamParams p) {
     __shared__ uint16_t s_beam[CAP];
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, group = blockIdx.x;
     const size_t row0 = (size_t)group * p.beams;
+    const uint64_t* list = p.list + row0 * p.pieces * p.len;
+    const uint32_t slots = p.beams * p.pieces * p.len;  // below 2^31
+    auto fetch = [&](uint32_t i0, uint64_t (&e)[JOIN_AT_ONCE]) {
+#pragma unroll
+        for (uint32_t u = 0; u < JOIN_AT_ONCE; ++u) e[u] = i0 + u * JOIN_THREADS < slots ? list[i0 + u * JOIN_THREADS] : 0;
+    };
+    uint64_t head[JOIN_AT_ONCE];  // the first entries: under way while the logs are taken, and kept
+    fetch(t, head);
     for (uint32_t b = wave; b < p.beams; b += JOIN_WAVES) {
         const size_t at = (row0 + b) * p.pieces;
+        const float start = p.scores ? p.scores[row0 + b] : 0.0f;
         double lse = 0.0;
         if (NORMALIZE && !(p.finished && p.finished[row0 + b])) {
             float m = -__builtin_inff();
             bool bad = false;
-            for (uint32_t i = lane; i < p.pieces; i += 64) {
-                const float v = p.peak[at + i];
-                bad |= v != v;
-                m = fmaxf(m, v);
-            }
-            for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-            bad = __any(bad) || m == __builtin_inff();
             double s = 0.0;
-            if (m > -__builtin_inff())
-                for (uint32_t i = lane; i < p.pieces; i += 64) s += p.sum[at + i] * exp64((double)p.peak[at + i] - (double)m);
+            for (uint32_t i0 = 0; i0 < p.pieces; i0 += 64) {  // (a row of more than 64 pieces: its sums are scaled as its maximum grows)
+                const bool in = i0 + lane < p.pieces;
+                const float v = in ? p.peak[at + i0 + lane] : -__builtin_inff();
+                const double part = in ? p.sum[at + i0 + lane] : 0.0;
+                bad |= v != v;
+                float most = fmaxf(m, v);
+                for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+                if (most > -__builtin_inff()) s = (m > -__builtin_inff() ? s * exp64((double)m - (double)most) : 0.0) + (v > -__builtin_inff() ? part * exp64((double)v - (double)most) : 0.0);
+                m = most;
+            }
+            bad = __any(bad) || m == __builtin_inff();
             s = wave_sum(s);
             lse = bad ? __longlong_as_double(0x7ff8000000000000ll) : (double)m + log(s);
         }
         if (lane == 0) {
             s_lse[b] = lse;
-            s_start[b] = p.scores ? p.scores[row0 + b] : 0.0f;
+            s_start[b] = start;
         }
     }
     if (t == 0) s_n = 0;
     if (t < 256 * GROUPS) s_max[t] = 0;
     __syncthreads();
-    const uint64_t* list = p.list + row0 * p.pieces * p.len;
-    const uint32_t slots = p.beams * p.pieces * p.len;  // below 2^31
     // order of the total and beam of a list entry; an ended beam's entry holds a logit of 0 and no sum
     auto total_of = [&](uint64_t e, uint32_t i, uint32_t* beam) -> uint64_t {
         const uint32_t b = (uint32_t)(((uint64_t)i * p.per_row_magic) >> (31 + p.per_row_shift));
@@ -463,13 +472,13 @@ __global__ __launch_bounds__(JOIN_THREADS) void beam_join_kernel(BeamParams p) {
     auto each = [&](auto f) {
         for (uint32_t i0 = t; i0 < slots; i0 += JOIN_THREADS * JOIN_AT_ONCE) {
             uint64_t e[JOIN_AT_ONCE];
-#pragma unroll
-            for (uint32_t u = 0; u < JOIN_AT_ONCE; ++u) e[u] = i0 + u * JOIN_THREADS < slots ? list[i0 + u * JOIN_THREADS] : 0;
+            if (i0 != t) fetch(i0, e);
 #pragma unroll
             for (uint32_t u = 0; u < JOIN_AT_ONCE; ++u) {
+                const uint64_t entry = i0 == t ? head[u] : e[u];
                 uint32_t beam = 0;
-                const uint64_t o = e[u] ? total_of(e[u], i0 + u * JOIN_THREADS, &beam) : 0;
-                if (o) f(o, e[u], beam, i0 + u * JOIN_THREADS);
+                const uint64_t o = entry ? total_of(entry, i0 + u * JOIN_THREADS, &beam) : 0;
+                if (o) f(o, entry, beam, i0 + u * JOIN_THREADS);
             }
         }
     };

@@ -54,13 +54,45 @@ def _wait_for_producer(t) -> None:
 
 
 _VALUES = {"torch.float32": _lib.VALUE_F32, "torch.float16": _lib.VALUE_F16, "torch.bfloat16": _lib.VALUE_BF16}
+_NAMES: dict = {}  # torch dtypes by the object: a name costs more than the rest of a check
+
+
+def _dtype(t) -> str:
+    name = _NAMES.get(t.dtype)
+    if name is None:
+        name = _NAMES[t.dtype] = str(t.dtype)
+    return name
 
 
 def _value(t, what: str) -> int:
-    v = _VALUES.get(str(t.dtype))
+    v = _VALUES.get(_dtype(t))
     if v is None:
         raise ValueError(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
     return v
+
+
+def _rows_of(t, name: str, dtype=None, cols=None, rows=None):
+    """(rows, columns, elements from row to row) of a matrix whose rows are contiguous, any distance apart."""
+    shape = t.shape
+    if len(shape) != 2 or (dtype is not None and _dtype(t) not in dtype) or (cols is not None and shape[1] != cols) or \
+            (rows is not None and shape[0] != rows):
+        raise ValueError(f"{name} must be [{'n' if rows is None else rows}, {'dim' if cols is None else cols}]"
+                         f"{'' if dtype is None else ' of ' + ' or '.join(dtype)}, not {list(shape)} of {t.dtype}")
+    n, dim = shape
+    apart, next_to = t.stride()
+    if n <= 1:
+        apart = dim
+    if (dim > 1 and next_to != 1) or apart < dim:
+        raise ValueError(f"{name} must have contiguous rows that do not overlap")
+    return n, dim, apart
+
+
+_F32, _I8, _WORDS, _FLAGS = ("torch.float32",), ("torch.int8",), ("torch.int32", "torch.uint32"), ("torch.bool", "torch.uint8")
+
+
+def _flat(t, name: str, dtype, size: int) -> None:
+    if _dtype(t) not in dtype or t.numel() != size or not t.is_contiguous():
+        raise ValueError(f"{name} must be {size} contiguous values of {' or '.join(dtype)}, not {list(t.shape)} of {t.dtype}")
 
 
 def _codes_i8(codes, scales, what: str):
@@ -266,31 +298,12 @@ class Context:
                                                            d_out_dists.data_ptr(), d_out_counts.data_ptr()))
 
     # ---- rows in 8-bit integers, their products, the best continuations ---------------------------------------------
-    def _check_device(self, **tensors) -> None:
+    def _check_device(self, *tensors) -> None:
         """Every given tensor lies on the context's device; the caller's stream there has finished."""
-        for name, t in tensors.items():
-            if t is not None and (not getattr(t, "is_cuda", False) or t.device.index != self.device):
-                raise ValueError(f"{name} must be a tensor on device {self.device}")
-        _wait_for_producer(next(t for t in tensors.values() if t is not None))
-
-    @staticmethod
-    def _check_rows(t, name: str, dtype=None, cols=None, rows=None) -> None:
-        """A matrix whose rows are contiguous (any stride between them)."""
-        if t.dim() != 2 or (dtype is not None and str(t.dtype) != dtype) or (cols is not None and int(t.shape[1]) != cols) or \
-                (rows is not None and int(t.shape[0]) != rows):
-            raise ValueError(f"{name} must be [{'n' if rows is None else rows}, {'dim' if cols is None else cols}]"
-                             f"{'' if dtype is None else ' of ' + dtype}, not {list(t.shape)} of {t.dtype}")
-        if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-            raise ValueError(f"{name} must have contiguous rows that do not overlap")
-
-    @staticmethod
-    def _check_flat(t, name: str, dtype: str, size: int) -> None:
-        if str(t.dtype) != dtype or int(t.numel()) != size or not t.is_contiguous():
-            raise ValueError(f"{name} must be {size} contiguous values of {dtype}, not {list(t.shape)} of {t.dtype}")
-
-    @staticmethod
-    def _stride(t) -> int:
-        return int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1])
+        for t in tensors:
+            if t is not None and (not t.is_cuda or t.device.index != self.device):
+                raise ValueError(f"a tensor lies on {t.device}, the context on device {self.device}")
+        _wait_for_producer(tensors[0])
 
     def quantize_rows(self, rows):
         """(codes int8 [n, dim], scales f32 [n]) of float32 or float16 host rows: symmetric, scale = max |x| * (1 / 127) per row in f32,
@@ -307,14 +320,13 @@ class Context:
     def quantize_rows_device(self, d_rows, d_codes, d_scales) -> None:
         """The same for a float32 / float16 / bfloat16 device matrix, into int8 [n, dim] codes and float32 [n] scales; rows may
         lie apart.  A row with a NaN or an infinity gets scale NaN and codes 0."""
-        self._check_rows(d_rows, "d_rows")
-        n, dim = int(d_rows.shape[0]), int(d_rows.shape[1])
+        n, dim, apart = _rows_of(d_rows, "d_rows")
         value = _value(d_rows, "d_rows")
-        self._check_rows(d_codes, "d_codes", "torch.int8", dim, n)
-        self._check_flat(d_scales, "d_scales", "torch.float32", n)
-        self._check_device(d_rows=d_rows, d_codes=d_codes, d_scales=d_scales)
-        _lib.check(_lib.lib().needle_hip_quantize_rows_i8_device(self._h, d_rows.data_ptr(), value, n, dim, self._stride(d_rows),
-                                                                 d_codes.data_ptr(), self._stride(d_codes), d_scales.data_ptr()))
+        _, _, codes_apart = _rows_of(d_codes, "d_codes", _I8, dim, n)
+        _flat(d_scales, "d_scales", _F32, n)
+        self._check_device(d_rows, d_codes, d_scales)
+        _lib.check(_lib.lib().needle_hip_quantize_rows_i8_device(self._h, d_rows.data_ptr(), value, n, dim, apart, d_codes.data_ptr(),
+                                                                 codes_apart, d_scales.data_ptr()))
 
     def matmul_i8(self, a, a_scales, b, b_scales, bias=None) -> np.ndarray:
         """f32 [m, n] of (a[i] . b[j]) * a_scales[i] * b_scales[j] (+ bias[j]) for int8 host codes [m, k] and [n, k]
@@ -342,25 +354,26 @@ class Context:
         self._product(d_x, None, d_b, d_b_scales, d_out, d_bias)
 
     def _product(self, d_a, d_a_scales, d_b, d_b_scales, d_out, d_bias) -> None:
-        self._check_rows(d_a, "the rows", None if d_a_scales is None else "torch.int8")
-        m, k = int(d_a.shape[0]), int(d_a.shape[1])
-        self._check_rows(d_b, "d_b", "torch.int8")
-        if int(d_b.shape[1]) != k:
-            raise _lib.DimensionMismatch(_lib.ERR_DIMENSION_MISMATCH, f"Dimension mismatch: {k} and {int(d_b.shape[1])}")
-        n = int(d_b.shape[0])
-        self._check_rows(d_out, "d_out", None, n, m)
+        m, k, a_apart = _rows_of(d_a, "the rows", None if d_a_scales is None else _I8)
+        n, b_k, b_apart = _rows_of(d_b, "d_b", _I8)
+        if b_k != k:
+            raise _lib.DimensionMismatch(_lib.ERR_DIMENSION_MISMATCH, f"Dimension mismatch: {k} and {b_k}")
+        _, _, out_apart = _rows_of(d_out, "d_out", None, n, m)
         out_value = _value(d_out, "d_out")
-        for t, name, size in ((d_a_scales, "d_a_scales", m), (d_b_scales, "d_b_scales", n), (d_bias, "d_bias", n)):
-            if t is not None:
-                self._check_flat(t, name, "torch.float32", size)
-        x_value = _value(d_a, "d_x") if d_a_scales is None else None
-        self._check_device(a=d_a, a_scales=d_a_scales, d_b=d_b, d_b_scales=d_b_scales, d_out=d_out, d_bias=d_bias)
-        right = (m, d_b.data_ptr(), self._stride(d_b), d_b_scales.data_ptr(), n, k, None if d_bias is None else d_bias.data_ptr(), out_value,
-                 d_out.data_ptr(), self._stride(d_out))
+        _flat(d_b_scales, "d_b_scales", _F32, n)
+        if d_bias is not None:
+            _flat(d_bias, "d_bias", _F32, n)
         if d_a_scales is None:
-            _lib.check(_lib.lib().needle_hip_linear_i8_device(self._h, d_a.data_ptr(), x_value, self._stride(d_a), *right))
+            x_value = _value(d_a, "d_x")
         else:
-            _lib.check(_lib.lib().needle_hip_matmul_i8_device(self._h, d_a.data_ptr(), self._stride(d_a), d_a_scales.data_ptr(), *right))
+            _flat(d_a_scales, "d_a_scales", _F32, m)
+        self._check_device(d_a, d_a_scales, d_b, d_b_scales, d_out, d_bias)
+        right = (m, d_b.data_ptr(), b_apart, d_b_scales.data_ptr(), n, k, None if d_bias is None else d_bias.data_ptr(), out_value,
+                 d_out.data_ptr(), out_apart)
+        if d_a_scales is None:
+            _lib.check(_lib.lib().needle_hip_linear_i8_device(self._h, d_a.data_ptr(), x_value, a_apart, *right))
+        else:
+            _lib.check(_lib.lib().needle_hip_matmul_i8_device(self._h, d_a.data_ptr(), a_apart, d_a_scales.data_ptr(), *right))
 
     def beam_select(self, logits, scores, k: int, *, beams: int, normalize: bool = True, mask=None, finished=None, end_token: int = 0):
         """(parents, tokens uint32, scores f32, all [groups, k], counts uint32 [groups]): the k best continuations of every group
@@ -401,35 +414,29 @@ class Context:
         [groups], unused places -1 / -1 / -inf.  states: (src, dst) or (src, dst, axis) pairs of tensors whose dimension
         `axis` (default 0) holds groups * beams rows in src and groups * k in dst; dst's rows become copies of their
         parents' (rows of unused places stay as they were)."""
-        self._check_rows(d_logits, "d_logits")
-        rows, vocab = int(d_logits.shape[0]), int(d_logits.shape[1])
+        rows, vocab, apart = _rows_of(d_logits, "d_logits")
         if beams < 1 or rows % beams:
             raise ValueError("d_logits must be [groups * beams, vocab]")
         groups, value = rows // beams, _value(d_logits, "d_logits")
         if d_scores is not None:
-            self._check_flat(d_scores, "d_scores", "torch.float32", rows)
-        if d_finished is not None and str(d_finished.dtype) not in ("torch.bool", "torch.uint8"):
-            raise ValueError("d_finished must be bool or uint8")
+            _flat(d_scores, "d_scores", _F32, rows)
         if d_finished is not None:
-            self._check_flat(d_finished, "d_finished", str(d_finished.dtype), rows)
-        for t, name, size in ((d_parents, "d_parents", groups * k), (d_tokens, "d_tokens", groups * k), (d_counts, "d_counts", groups)):
-            self._check_flat(t, name, "torch.uint32" if str(t.dtype) == "torch.uint32" else "torch.int32", size)
-        self._check_flat(d_out_scores, "d_out_scores", "torch.float32", groups * k)
+            _flat(d_finished, "d_finished", _FLAGS, rows)
+        _flat(d_parents, "d_parents", _WORDS, groups * k)
+        _flat(d_tokens, "d_tokens", _WORDS, groups * k)
+        _flat(d_counts, "d_counts", _WORDS, groups)
+        _flat(d_out_scores, "d_out_scores", _F32, groups * k)
         stride = 0
         if d_mask is not None:
-            words = (vocab + 31) // 32
-            one = d_mask.reshape(1, -1) if d_mask.dim() == 1 else d_mask
-            self._check_rows(one, "d_mask", "torch.uint32" if str(d_mask.dtype) == "torch.uint32" else "torch.int32", words)
-            if int(one.shape[0]) not in (1, rows):
+            n, _, words_apart = _rows_of(d_mask.reshape(1, -1) if d_mask.dim() == 1 else d_mask, "d_mask", _WORDS, (vocab + 31) // 32)
+            if n not in (1, rows):
                 raise ValueError("d_mask must have one row, or one for every row of d_logits")
-            stride = self._stride(one) if int(one.shape[0]) == rows and rows > 1 else 0
-        arr, n_states = self._states(states, groups, beams, k)
-        self._check_device(d_logits=d_logits, d_scores=d_scores, d_mask=d_mask, d_finished=d_finished, d_parents=d_parents,
-                           d_tokens=d_tokens, d_out_scores=d_out_scores, d_counts=d_counts)
-        p = _lib.BeamParams(groups=groups, beams=beams, vocab=vocab, k=k, value=value, normalize=int(bool(normalize)),
-                            row_stride=self._stride(d_logits), scores=None if d_scores is None else d_scores.data_ptr(),
-                            finished=None if d_finished is None else d_finished.data_ptr(),
-                            mask=None if d_mask is None else d_mask.data_ptr(), mask_stride=stride, end_token=end_token, reserved=0)
+            stride = words_apart if n == rows and rows > 1 else 0
+        arr, n_states = self._states(states, groups, beams, k) if states else (None, 0)
+        self._check_device(d_logits, d_scores, d_mask, d_finished, d_parents, d_tokens, d_out_scores, d_counts)
+        p = _lib.BeamParams(groups, beams, vocab, k, value, 1 if normalize else 0, apart, None if d_scores is None else d_scores.data_ptr(),
+                            None if d_finished is None else d_finished.data_ptr(), None if d_mask is None else d_mask.data_ptr(), stride,
+                            end_token, 0)
         _lib.check(_lib.lib().needle_hip_beam_select_device(self._h, C.byref(p), d_logits.data_ptr(), arr, n_states, d_parents.data_ptr(),
                                                             d_tokens.data_ptr(), d_out_scores.data_ptr(), d_counts.data_ptr()))
 
@@ -439,9 +446,9 @@ class Context:
         if d_parents.dim() != 2 or beams < 1:
             raise ValueError("d_parents must be [groups, k]")
         groups, k = int(d_parents.shape[0]), int(d_parents.shape[1])
-        self._check_flat(d_parents, "d_parents", "torch.uint32" if str(d_parents.dtype) == "torch.uint32" else "torch.int32", groups * k)
+        _flat(d_parents, "d_parents", _WORDS, groups * k)
         arr, n_states = self._states(states, groups, beams, k)
-        self._check_device(d_parents=d_parents)
+        self._check_device(d_parents)
         _lib.check(_lib.lib().needle_hip_beam_reorder_device(self._h, d_parents.data_ptr(), groups, beams, k, arr, n_states))
 
     def _states(self, states, groups: int, beams: int, k: int):
