@@ -181,6 +181,7 @@ struct MatmulParams {
     void* out;
     uint64_t a_stride, b_stride, out_stride, n;
     uint32_t m, k;
+    uint32_t past;  // the output does not fit the memory-side cache and its rows start on 64 bytes: it goes past it
 };
 
 // 16 codes of a row from place `at` on, zero from k on; nothing outside the row is read.  The last codes of a row are the
@@ -505,7 +506,14 @@ __global__ __launch_bounds__(64 * WB * WA) void matmul_i8_tile_kernel(MatmulPara
             for (int g = 0; g < ROWS / GO; ++g) {
                 const uint32_t r = g * GO + lane / CHUNKS, c = lane % CHUNKS;
                 const u32x4 v = *(const u32x4*)(part + r * LINE + ((c ^ r) & (CHUNKS - 1)) * 16);
-                *(u32x4_any*)((uint8_t*)(o + (uint64_t)(y0 * 16 + r) * p.out_stride) + c * 16) = v;
+                u32x4_any* to = (u32x4_any*)((uint8_t*)(o + (uint64_t)(y0 * 16 + r) * p.out_stride) + c * 16);
+                if (p.past) {
+                    asm volatile("");  // (without these the compiler makes one ordinary store of the two)
+                    __builtin_nontemporal_store(v, to);
+                    asm volatile("");
+                } else {
+                    *to = v;
+                }
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -539,15 +547,30 @@ static hipError_t launch_tiles_of(const MatmulParams& p, hipStream_t stream) {
     hipLaunchKernelGGL((matmul_i8_tile_kernel<V, TB, TA, WB, WA, SLOTS, DMA>), dim3(tiles_b * tiles_a), dim3(64 * WB * WA), lds, stream, p, tiles_b, tiles_a);
     return hipGetLastError();
 }
+constexpr uint64_t ALIGN_MOST = 2ull << 30;  // workspace of the aligned copies; beyond it the rows pass through registers
+// Rows of k codes copied to rows of `to_stride` (a multiple of 64) with zeros behind them, a wave per row.
+__global__ __launch_bounds__(256) void align_rows_kernel(const int8_t* __restrict__ rows, uint64_t n, uint32_t k, uint64_t stride,
+                                                         int8_t* __restrict__ to, uint32_t to_stride) {
+    const uint64_t row = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= n) return;
+    for (uint32_t at = (threadIdx.x & 63) * 16; at < to_stride; at += 1024) *(u32x4*)(to + row * to_stride + at) = load_codes(rows + row * stride, at, k);
+}
+
 template <typename V, int NB, int NA, bool SPLIT>
 static hipError_t launch_stream_of(const MatmulParams& p, hipStream_t stream) {
     const uint64_t tiles = (p.n + 16 * NB - 1) / (16 * NB);
     hipLaunchKernelGGL((matmul_i8_stream_kernel<V, NB, NA, SPLIT>), dim3((uint32_t)(SPLIT ? tiles : (tiles + 3) / 4)), dim3(256), 0, stream, p);
     return hipGetLastError();
 }
+static bool rows_aligned(const MatmulParams& p) {
+    return p.k % 16 == 0 && p.a_stride % 16 == 0 && p.b_stride % 16 == 0 && (uintptr_t)p.a % 16 == 0 && (uintptr_t)p.b % 16 == 0;
+}
+static bool fills_big_tiles(const MatmulParams& p, int n_cu) {
+    return p.m > 128 && p.k >= 512 && ((p.n + 255) / 256) * ((p.m + 255) / 256) >= (uint64_t)n_cu;
+}
 template <typename V>
 static hipError_t launch_matmul_of(const MatmulParams& p, int n_cu, hipStream_t stream) {
-    const bool aligned = p.k % 16 == 0 && p.a_stride % 16 == 0 && p.b_stride % 16 == 0 && (uintptr_t)p.a % 16 == 0 && (uintptr_t)p.b % 16 == 0;
+    const bool aligned = rows_aligned(p);
     if (p.m <= 16) {
         // split: long rows of a short table.  Otherwise many short-lived waves of one tile each hide the latency best.
         const bool split = p.n < 256ull * n_cu && p.k > 256;
@@ -561,7 +584,7 @@ static hipError_t launch_matmul_of(const MatmulParams& p, int n_cu, hipStream_t 
     // 64 x 64, 25 with 128 x 128).
     const auto tiles = [&](uint64_t tb, uint64_t ta) { return ((p.n + tb - 1) / tb) * ((p.m + ta - 1) / ta); };
     const uint64_t cu = (uint64_t)n_cu;
-    if (p.m > 128 && tiles(256, 256) >= cu && p.k >= 512)
+    if (fills_big_tiles(p, n_cu))
         return aligned ? launch_tiles_of<V, 256, 256, 2, 4, 4, true>(p, stream) : launch_tiles_of<V, 256, 128, 4, 2, 4, false>(p, stream);
     if (p.m > 64 && tiles(128, 128) >= cu / 2)
         return aligned ? launch_tiles_of<V, 128, 128, 4, 2, 4, true>(p, stream) : launch_tiles_of<V, 128, 128, 4, 2, 4, false>(p, stream);
@@ -569,11 +592,32 @@ static hipError_t launch_matmul_of(const MatmulParams& p, int n_cu, hipStream_t 
         return aligned ? launch_tiles_of<V, 128, 64, 2, 2, 4, true>(p, stream) : launch_tiles_of<V, 128, 64, 2, 2, 4, false>(p, stream);
     return aligned ? launch_tiles_of<V, 64, 64, 2, 2, 4, true>(p, stream) : launch_tiles_of<V, 64, 64, 2, 2, 4, false>(p, stream);
 }
-static hipError_t launch_matmul_i8(const MatmulParams& p, int out_value, int n_cu, hipStream_t stream) {
+static hipError_t launch_matmul_i8(needle_hip_ctx* c, MatmulParams p, int out_value) {
+    // 1000 x 100000 x 128 to 400 MB of f32: 81 us past the cache, 103 through it; to 134 MB of bf16 (8192 x 8192 x 64) 37 and
+    // 32; where rows do not start on 64 bytes (1000 x 100003) 190 and 106.
+    const uint64_t size = value_size(out_value);
+    p.past = p.m * p.n * size > (256ull << 20) && (uintptr_t)p.out % 64 == 0 && p.out_stride * size % 64 == 0;
+    // A long product of rows that the loads cannot write to LDS themselves (odd k, strides or addresses) copies them to
+    // aligned rows first: 8192 x 8192 x 1000 of odd strides takes 104 us with the copies, 145 through registers;
+    // 8192 x 9700 x 4001 343 and 518; 300 x 66000 x 513, too few rows of a for the copy of b to pay, 69 and 46.
+    if (p.m >= 1024 && fills_big_tiles(p, c->n_cu) && !rows_aligned(p)) {
+        const uint32_t stride = (p.k + 63) / 64 * 64;
+        const uint64_t bytes = (p.n + p.m) * stride;
+        if (bytes <= ALIGN_MOST) {
+            const hipError_t e = c->scratch[5].ensure(bytes);
+            if (e != hipSuccess) return e;
+            int8_t* to = c->scratch[5].as<int8_t>();
+            hipLaunchKernelGGL(align_rows_kernel, dim3((uint32_t)((p.n + 3) / 4)), dim3(256), 0, c->stream, p.b, p.n, p.k, p.b_stride, to, stride);
+            hipLaunchKernelGGL(align_rows_kernel, dim3((p.m + 3) / 4), dim3(256), 0, c->stream, p.a, (uint64_t)p.m, p.k, p.a_stride, to + p.n * stride, stride);
+            p.b = to;
+            p.a = to + p.n * stride;
+            p.a_stride = p.b_stride = p.k = stride;
+        }
+    }
     switch (out_value) {
-    case NEEDLE_VALUE_F32: return launch_matmul_of<ValueF32>(p, n_cu, stream);
-    case NEEDLE_VALUE_F16: return launch_matmul_of<ValueF16>(p, n_cu, stream);
-    default: return launch_matmul_of<ValueBF16>(p, n_cu, stream);
+    case NEEDLE_VALUE_F32: return launch_matmul_of<ValueF32>(p, c->n_cu, c->stream);
+    case NEEDLE_VALUE_F16: return launch_matmul_of<ValueF16>(p, c->n_cu, c->stream);
+    default: return launch_matmul_of<ValueBF16>(p, c->n_cu, c->stream);
     }
 }
 
@@ -674,8 +718,8 @@ extern "C" needle_hip_status needle_hip_matmul_i8_device(needle_hip_ctx* c, cons
     std::lock_guard g(c->mu);
     DeviceScope dev(c->device);
     HIP_TRY(dev.error());
-    const MatmulParams p{d_a, d_b, d_a_scales, d_b_scales, d_bias, d_out, a_stride, b_stride, out_stride, n, m, k};
-    HIP_TRY(launch_matmul_i8(p, out_value, c->n_cu, c->stream));
+    const MatmulParams p{d_a, d_b, d_a_scales, d_b_scales, d_bias, d_out, a_stride, b_stride, out_stride, n, m, k, 0};
+    HIP_TRY(launch_matmul_i8(c, p, out_value));
     HIP_TRY(hipStreamSynchronize(c->stream));
     return NEEDLE_HIP_OK;
 }
@@ -696,8 +740,8 @@ extern "C" needle_hip_status needle_hip_matmul_i8(needle_hip_ctx* c, const int8_
     for (int i = 0; i < 5; ++i)
         if (sizes[i]) HIP_TRY(hipMemcpyAsync(d + at[i], src[i], sizes[i], hipMemcpyHostToDevice, c->stream));
     const MatmulParams p{(const int8_t*)(d + at[0]), (const int8_t*)(d + at[1]), (const float*)(d + at[2]), (const float*)(d + at[3]),
-                         bias ? (const float*)(d + at[4]) : nullptr, d + at[5], k, k, n, n, m, k};
-    HIP_TRY(launch_matmul_i8(p, NEEDLE_VALUE_F32, c->n_cu, c->stream));
+                         bias ? (const float*)(d + at[4]) : nullptr, d + at[5], k, k, n, n, m, k, 0};
+    HIP_TRY(launch_matmul_i8(c, p, NEEDLE_VALUE_F32));
     HIP_TRY(hipMemcpyAsync(out, d + at[5], sizes[5], hipMemcpyDeviceToHost, c->stream));
     HIP_TRY(hipStreamSynchronize(c->stream));
     return NEEDLE_HIP_OK;
@@ -718,8 +762,8 @@ extern "C" needle_hip_status needle_hip_linear_i8_device(needle_hip_ctx* c, cons
     int8_t* d_codes = c->scratch[6].as<int8_t>();
     float* d_scales = (float*)(d_codes + (size_t)m * stride);
     HIP_TRY(launch_quantize_rows(d_x, x_value, m, k, x_stride, d_codes, stride, d_scales, c->stream));
-    const MatmulParams p{d_codes, d_b, d_scales, d_b_scales, d_bias, d_out, stride, b_stride, out_stride, n, m, k};
-    HIP_TRY(launch_matmul_i8(p, out_value, c->n_cu, c->stream));
+    const MatmulParams p{d_codes, d_b, d_scales, d_b_scales, d_bias, d_out, stride, b_stride, out_stride, n, m, k, 0};
+    HIP_TRY(launch_matmul_i8(c, p, out_value));
     HIP_TRY(hipStreamSynchronize(c->stream));
     return NEEDLE_HIP_OK;
 }

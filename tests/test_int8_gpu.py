@@ -226,10 +226,10 @@ def test_matmul_behind_four_billion(ctx, torch):
     """Outputs and rows whose offsets pass 32 bits."""
     g = torch.Generator(device="cuda").manual_seed(5)
     a, sa = _table(torch, g, 70_000, 16)
-    b, sb = _table(torch, g, 66_000, 16)
-    out = torch.empty(70_000, 66_000, dtype=torch.bfloat16, device="cuda")
+    b, sb = _table(torch, g, 66_048, 16)
+    out = torch.empty(70_000, 66_048, dtype=torch.bfloat16, device="cuda")
     ctx.matmul_i8_device(a, sa, b, sb, out)
-    for r, c in ((slice(0, 65), slice(0, 65)), (slice(69_900, 70_000), slice(65_900, 66_000)), (slice(65_100, 65_200), slice(30_000, 30_100))):
+    for r, c in ((slice(0, 65), slice(0, 65)), (slice(69_900, 70_000), slice(65_900, 66_048)), (slice(65_100, 65_200), slice(30_000, 30_100))):
         _check_product(out[r, c], a[r], sa[r], b[c], sb[c], None, "bfloat16")
     del out
     wide = torch.randint(-127, 128, (3, 2 ** 31 + 64), generator=g, device="cuda", dtype=torch.int8)  # rows 2 GiB apart
