@@ -107,27 +107,26 @@ def _state_layout(src, dst, axis: int):
     """(outer, inner, bytes, strides of src, strides of dst) in bytes of two tensors whose dimension `axis` numbers the
     rows: dimensions before it must fold into one, those behind it into runs of neighbouring elements that lie one stride
     apart."""
-    def fold(dims):  # [(size, src stride, dst stride)]: neighbours that continue each other in both tensors become one
-        out = []
-        for n, a, b in dims:
-            if n == 1:
+    shape, a, b, size = tuple(src.shape), src.stride(), dst.stride(), src.element_size()
+    run, i = 1, len(shape) - 1
+    while i > axis and (shape[i] == 1 or a[i] == b[i] == run):  # dimensions that continue the run in both tensors
+        run *= shape[i]
+        i -= 1
+    parts = []
+    for first, last in ((i, axis), (axis - 1, -1)):  # behind the rows, then before them
+        n, sa, sb = 1, 0, 0
+        for d in range(first, last, -1):
+            if shape[d] == 1:
                 continue
-            if out and out[-1][1] == n * a and out[-1][2] == n * b:
-                out[-1] = (out[-1][0] * n, a, b)
+            if n == 1:
+                n, sa, sb = shape[d], a[d], b[d]
+            elif a[d] == n * sa and b[d] == n * sb:
+                n *= shape[d]
             else:
-                out.append((n, a, b))
-        return out
-
-    size = src.element_size()
-    dims = [(int(n), int(a) * size, int(b) * size) for n, a, b in zip(src.shape, src.stride(), dst.stride())]
-    before, behind = fold(dims[:axis]), fold(dims[axis + 1:])
-    run = size
-    if behind and behind[-1][1] == behind[-1][2] == size:
-        run *= behind.pop()[0]
-    if len(before) > 1 or len(behind) > 1:
-        raise ValueError("a state's dimensions must fold into one before its rows and, behind them, into runs one stride apart")
-    outer, inner = before[0] if before else (1, 0, 0), behind[0] if behind else (1, 0, 0)
-    return outer[0], inner[0], run, (outer[1], int(src.stride(axis)) * size, inner[1]), (outer[2], int(dst.stride(axis)) * size, inner[2])
+                raise ValueError("a state's dimensions must fold into one before its rows and, behind them, into runs one stride apart")
+        parts.append((n, sa * size, sb * size))
+    (inner, ia, ib), (outer, oa, ob) = parts
+    return outer, inner, run * size, (oa, a[axis] * size, ia), (ob, b[axis] * size, ib)
 
 
 def _destroy_handle(owner, destroy_name: str = "needle_hip_index_destroy") -> None:
@@ -301,7 +300,7 @@ class Context:
     def _check_device(self, *tensors) -> None:
         """Every given tensor lies on the context's device; the caller's stream there has finished."""
         for t in tensors:
-            if t is not None and (not t.is_cuda or t.device.index != self.device):
+            if t is not None and t.get_device() != self.device:  # -1 on the host
                 raise ValueError(f"a tensor lies on {t.device}, the context on device {self.device}")
         _wait_for_producer(tensors[0])
 
@@ -456,20 +455,18 @@ class Context:
         for s in states:
             src, dst = s[0], s[1]
             axis = s[2] if len(s) > 2 else 0
-            if src.dtype != dst.dtype or src.dim() != dst.dim() or not 0 <= axis < src.dim() or \
-                    any(a != b for i, (a, b) in enumerate(zip(src.shape, dst.shape)) if i != axis):
-                raise ValueError("a state's src and dst must differ in nothing but their rows")
-            if int(src.shape[axis]) != groups * beams or int(dst.shape[axis]) != groups * k:
+            here, there = list(src.shape), list(dst.shape)
+            if not 0 <= axis < len(here) or here[axis] != groups * beams or len(there) != len(here) or there[axis] != groups * k:
                 raise ValueError(f"a state must have {groups * beams} rows in src and {groups * k} in dst")
-            for t in (src, dst):
-                if not t.is_cuda or t.device.index != self.device:
-                    raise ValueError(f"states must be tensors on device {self.device}")
+            here[axis] = there[axis] = 0
+            if here != there or src.dtype != dst.dtype:
+                raise ValueError("a state's src and dst must differ in nothing but their rows")
+            if src.get_device() != self.device or dst.get_device() != self.device:
+                raise ValueError(f"states must be tensors on device {self.device}")
             if src.numel() == 0 or dst.numel() == 0:
                 continue
             outer, inner, run, a, b = _state_layout(src, dst, axis)
-            out.append(_lib.BeamState(src=src.data_ptr(), dst=dst.data_ptr(), outer=outer, inner=inner, bytes=run,
-                                      src_outer_stride=a[0], src_row_stride=a[1], src_inner_stride=a[2],
-                                      dst_outer_stride=b[0], dst_row_stride=b[1], dst_inner_stride=b[2]))
+            out.append(_lib.BeamState(src.data_ptr(), dst.data_ptr(), outer, inner, run, *a, *b))
         return ((_lib.BeamState * len(out))(*out) if out else None), len(out)
 
 

@@ -240,10 +240,13 @@ def test_matmul_behind_four_billion(ctx, torch):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("m,n,k", [(1, 40, 33), (4, 1000, 1024), (37, 130, 301), (300, 520, 768), (2, 3, 0)])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 33), (4, 1000, 1024), (37, 130, 301), (300, 520, 768), (2, 3, 0), (1, 8192, 8192), (16, 300, 511), (5, 17_000, 300),
+                                   (13, 33_000, 630), (3, 1, 2047), (16, 70_000, 400), (2, 4099, 4096)])
 def test_linear_is_quantize_then_matmul(ctx, torch, dtype, m, n, k):
     g = torch.Generator(device="cuda").manual_seed(m + n)
     x = torch.randn(m, k + 3, generator=g, device="cuda").to(getattr(torch, dtype))[:, :k]
+    if m > 4:
+        x[1], x[3, k // 2] = 0, float("inf")
     b, sb = _table(torch, g, n, k)
     bias = torch.randn(n, generator=g, device="cuda")
     for out_dtype in (torch.float32, x.dtype):
@@ -251,7 +254,9 @@ def test_linear_is_quantize_then_matmul(ctx, torch, dtype, m, n, k):
         ctx.linear_i8_device(x, b, sb, out, d_bias=bias)
         codes, scales = _quantize(torch, ctx, x)
         ctx.matmul_i8_device(codes, scales, b, sb, two, d_bias=bias)
-        assert torch.equal(out, two)
+        assert torch.equal(out.isnan(), two.isnan()) and torch.equal(out.nan_to_num(7.0), two.nan_to_num(7.0))
+        if m > 4:
+            assert out[3].isnan().all() and torch.equal(out[1].float(), bias.to(out_dtype).float())
 
 
 def test_matmul_host_form(ctx):
