@@ -540,7 +540,7 @@ needle_hip_status needle_hip_quantize_rows_i8_device(needle_hip_ctx* ctx, const 
  * guarantees for any codes (-128 included); it is turned into f32, multiplied by the
  * two scales in that order, the bias (nullable) is added, and the result is rounded once
  * more where out_value (needle_value) is a half type.  k may be a prefix of longer rows (stride
- * above k).  m * n may be any size, n < 2^31.  k 0 gives the bias, or zeros. */
+ * above k).  m, n < 2^31; m * n may be any size.  k 0 gives the bias, or zeros. */
 needle_hip_status needle_hip_matmul_i8(needle_hip_ctx* ctx, const int8_t* a, const float* a_scales, uint32_t m,
                                        const int8_t* b, const float* b_scales, uint64_t n, uint32_t k,
                                        const float* bias, float* out);
@@ -567,7 +567,8 @@ needle_hip_status needle_hip_linear_i8_device(needle_hip_ctx* ctx, const void* d
  * NaN (so a beam whose score is -inf or NaN offers nothing; nor does, under normalize, a
  * row with an admitted NaN or +inf).  An ended beam offers one continuation: end_token
  * with scores[row] as its total; its row of logits and its mask are not looked at.
- * k <= 256, beams <= 1024, beams * vocab < 2^32, groups * beams < 2^31. */
+ * k <= 256, beams <= 1024, vocab < 2^31, beams * vocab < 2^32, groups * beams and
+ * groups * k < 2^31. */
 typedef struct needle_beam_params {
     uint32_t groups, beams, vocab, k;
     int32_t value;            /* needle_value of the logits */
@@ -584,7 +585,8 @@ typedef struct needle_beam_params {
 /* Something every beam carries (keys and values, a query vector, a history): after the
  * picks, row g * k + j of dst becomes a copy of row g * beams + parent of src.  A row is
  * outer x inner runs of `bytes` bytes; all strides are in bytes.  Rows of places without
- * a pick stay as they were.  dst must not overlap any src or another dst. */
+ * a pick stay as they were.  dst must not overlap any src, another dst or another array
+ * of the call. */
 typedef struct needle_beam_state {
     const void* src;
     void* dst;

@@ -7,11 +7,11 @@
 // keeps, per piece of a row, its maximum, its sum of exponentials and its k largest logits; a second, small kernel joins the
 // pieces of a group.  The pass is bound by the bytes of the logits.
 //
-// Picks are whole numbers and two beams' totals may lie a rounding apart, so what decides between beams is held in 64 bits:
-// the totals, the sums, and the exponentials of the logits that may be picked -- they are the large terms of a sum.  The
-// many small terms are taken in f32 by a polynomial whose error (3e-8 of a term, mean 1.3e-9) averages out over them: an
-// f64 instruction takes twice the cycles of an f32 one here, and eight f64 ones per logit bound the kernel (73 us for 64 x 8
-// rows of 131072 bf16 logits).
+// Picks are whole numbers and two beams' totals may lie a rounding apart, so all that decides between beams is held in 64
+// bits: the exponentials, their sums, the totals.  An f64 instruction takes twice the cycles of an f32 one here, and about
+// fourteen of them per logit bound the kernel where it takes a log-softmax of half-precision logits (70 us for 64 x 8 rows
+// of 131072 bf16 logits; an f32 polynomial for all but the largest terms took 60 us, and erred by 1e-7 in the log where
+// thousands of logits are equal).
 #include "nh_values.h"
 
 namespace nh {
@@ -37,24 +37,6 @@ __device__ inline double exp64(double x) {
     p = __builtin_fma(p, f, 0x1.62e42fef9cc69p-1);
     p = __builtin_fma(p, f, 0x1.ffffffffa7135p-1);
     return __hiloint2double(__double2hiint(p) + (__double2loint(s) << 20), __double2loint(p));
-}
-
-// exp x in units of 2^nref, for |x| < 2^20 and x / ln 2 - nref > -120, in f32: 2^f by a polynomial of degree 6 through the
-// seven Chebyshev nodes of |f| <= 1/2.  `shift` = 1.5 * 2^23 - nref, so that the sum with x / ln 2 holds n - nref in its low
-// bits; the two multiply-adds keep f to 2^-26 however large n is.
-__device__ inline float exp32_scaled(float x, float shift) {
-    constexpr float HI = 0x1.715476p+0f, LO = 0x1.4ae0cp-26f;  // 1 / ln 2
-    const float s = __builtin_fmaf(x, HI, shift), n = s - shift;
-    float f = __builtin_fmaf(x, HI, -n);
-    f = __builtin_fmaf(x, LO, f);
-    float p = 0x1.444p-13f;
-    p = __builtin_fmaf(p, f, 0x1.5f48cp-10f);
-    p = __builtin_fmaf(p, f, 0x1.3b2a1cp-7f);
-    p = __builtin_fmaf(p, f, 0x1.c6aeccp-5f);
-    p = __builtin_fmaf(p, f, 0x1.ebfbep-3f);
-    p = __builtin_fmaf(p, f, 0x1.62e43p-1f);
-    p = __builtin_fmaf(p, f, 1.0f);
-    return __uint_as_float(__float_as_uint(p) + (__float_as_uint(s) << 23));
 }
 
 // order-preserving whole number of a double (-0 as +0); 0 for what is never offered (-inf, NaN)
@@ -146,11 +128,12 @@ struct BeamParams {
 // k-th largest of GROUPS running maxima per thread, which k logits reach; it is found again after 1, 2, 4, 8, ... chunks, so
 // that about k log2(chunks) logits are listed in all.  Which logits a thread adds up, and in which order, follows from the
 // places and values of its row alone: equal rows have equal sums.
+//
+// Not normalized it is bound by the bytes: 32 x 10 x 100003 f32, k = 64, take 30 us (4.3 TB/s).
 template <typename V, int EACH, int GROUPS, bool NORMALIZE, bool MASKED>
 __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p) {
     constexpr int WIDE = 16 / V::size, LOADS = EACH / WIDE, CAP = 1024, MINE = CAP / PIECE_THREADS;
     constexpr uint32_t CHUNK = PIECE_THREADS * EACH, LOWEST = 0x00800000u;  // LOWEST: order of the lowest finite f32
-    constexpr double LN2 = 0.69314718055994530942;
     __shared__ uint32_t s_max[PIECE_THREADS * GROUPS];
     __shared__ __align__(16) uint64_t s_list[CAP + 8];
     __shared__ double s_sum[4];
@@ -199,8 +182,8 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) run[g] = -__builtin_inff();
     // the thread's sum of exponentials, in units of exp(unit) = 2^nref where the f32 path applies
-    double sum = 0.0, unit = 0.0;
-    float ref = -__builtin_inff(), shift = 0.0f;
+    double sum = 0.0;
+    float ref = -__builtin_inff();
     bool nan = false;
     uint32_t slot = 0;
 
@@ -271,8 +254,6 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
             const float b = raise();
             bound = done == 1 ? b : fmaxf(bound, b);
         }
-        const float listed = bound;
-        const bool any = __any(top >= listed);
         // the logits that reach `least` go behind the list's n entries: one place per wave, then one per logit; how many
         auto append = [&](float least) {
             if (__any(top >= least)) {
@@ -302,13 +283,14 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
             slot = slot == 2 ? 0 : slot + 1;
             return add;
         };
-        uint32_t add = append(listed);
+        uint32_t add = append(bound);
         if (n + add > CAP) {
             // Large logits that come late in the row: this chunk raises the bound itself.  If thousands still reach it
             // (equal ones, or an order that puts all large ones into few threads), one logit of every thread at a time
             // goes to the list, which is cut back as it fills.
             bound = fmaxf(bound, raise());
             add = 0;
+            if (n > CAP - PIECE_THREADS && cut()) bound = fmaxf(bound, ord2f((uint32_t)(s_list[n - 1] >> 32)));  // room for one of every thread
             if (t == 0) s_fill = n;
             __syncthreads();
 #pragma unroll 1
@@ -334,43 +316,16 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
         }
         n += add;
         if (NORMALIZE && top > -__builtin_inff()) {
-            if (!(top - ref <= 20.0f)) {  // ref is -inf at first
-                const bool started = ref > -__builtin_inff();
-                const double was = unit;
+            if (!(top - ref <= 64.0f)) {  // ref is -inf at first
+                sum = ref > -__builtin_inff() ? sum * exp64((double)ref - (double)top) : 0.0;
                 ref = top;
-                const float nref = rintf(ref * 1.44269504f);
-                shift = 12582912.0f - nref;  // 1.5 * 2^23
-                unit = fabsf(ref) < 0x1p20f ? (double)nref * LN2 : (double)ref;
-                sum = started ? sum * exp64(was - unit) : 0.0;
             }
-            const bool small = fabsf(ref) < 0x1p20f;
-            // In 64 bits, one logit of every thread at a time: what the list got, or all of them where f32 has no digits left.
-            if (any || __any(!small)) {
-                uint32_t left = 0;
-#pragma unroll
-                for (int e = 0; e < EACH; ++e) left |= v[e] >= (small ? listed : -3.40282347e+38f) ? 1u << e : 0;
-#pragma unroll 1
-                while (__any(left != 0)) {
-                    const uint32_t e0 = left ? (uint32_t)__builtin_ctz(left) : ~0u;
-                    float y = -__builtin_inff();
-#pragma unroll
-                    for (int e = 0; e < EACH; ++e)
-                        if (e0 == (uint32_t)e) {
-                            y = v[e];
-                            v[e] = -__builtin_inff();
-                        }
-                    if (left) sum += exp64((double)y - unit);
-                    left &= left - 1;
-                }
-            }
-            const float least = ref - 80.0f;  // e^-80 beside a term of 1 is nothing
-            float part = 0.0f;
+            const double r = (double)ref;
 #pragma unroll
             for (int e = 0; e < EACH; ++e) {
-                part += exp32_scaled(fmaxf(v[e], least), shift);
+                sum += exp64((double)v[e] - r);
                 if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: more in flight cost registers, and waves
             }
-            if (small) sum += (double)part;
         }
         if (!more) break;
     }
@@ -383,7 +338,7 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
         if (nan) s_nan = 1;
         __syncthreads();
         m = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-        sum = ref > -__builtin_inff() ? sum * exp64(unit - (double)m) : 0.0;
+        sum = ref > -__builtin_inff() ? sum * exp64((double)ref - (double)m) : 0.0;
         sum = wave_sum(sum);
         if (lane == 0) s_sum[wave] = sum;
         __syncthreads();
@@ -641,10 +596,11 @@ static hipError_t launch_moves(const uint32_t* d_parents, uint32_t groups, uint3
 }
 
 // ---- host side ---------------------------------------------------------------------------------
-// Bytes of a row per thread and chunk.  64 x 8 rows of 131072 bf16 logits: 59 us with 32 (114 registers, four workgroups
-// per CU), 80 us with 64 (164 registers, three).
+// Bytes of a row per thread and chunk: 64 x 8 rows of 131072 bf16 logits take a third longer with 64, whose registers leave
+// room for three workgroups per CU.
 constexpr uint32_t LONG_BYTES = 32;
-// Workgroups per CU that the pieces are cut for: the same rows take 59 us with 4, 72 us with 5, 70 us with 8, 78 us with 16.
+// Workgroups per CU that the pieces are cut for: the same rows take 70 us
+// with 4, 76 with 5, 73 with 8; 32 x 10 rows of 100003 f32 logits, not normalized, 30, 30 and 33.
 constexpr uint32_t PIECES_PER_CU = 4;
 template <typename V, int EACH, int GROUPS>
 static void launch_pieces_of(const BeamParams& p, bool normalize, hipStream_t stream) {
@@ -667,7 +623,10 @@ static void launch_pieces(const BeamParams& p, bool normalize, bool short_chunks
     }
 }
 
-static needle_hip_status states_check(const needle_beam_state* states, uint32_t n_states, uint64_t rows, uint64_t picks) {
+struct ByteRange { const void* p; uint64_t n; };
+// `others`: arrays of the same call that no dst may overlap
+static needle_hip_status states_check(const needle_beam_state* states, uint32_t n_states, uint64_t rows, uint64_t picks, const ByteRange* others,
+                                      int n_others) {
     if (n_states && !states) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "states is null");
     if (n_states > STATES_MAX) return fail(NEEDLE_HIP_ERR_UNSUPPORTED, "at most %u states per call", STATES_MAX);
     struct Range { uint64_t first, second; } from[STATES_MAX] = {}, to[STATES_MAX] = {};  // first byte, last byte + 1
@@ -692,6 +651,9 @@ static needle_hip_status states_check(const needle_beam_state* states, uint32_t 
                 return fail(NEEDLE_HIP_ERR_UNSUPPORTED, "state %u spans more than 2^62 bytes", i);
         from[i] = {(uint64_t)s.src, (uint64_t)s.src + reach};
         to[i] = {(uint64_t)s.dst, (uint64_t)s.dst + span};
+        for (int o = 0; o < n_others; ++o)
+            if (ranges_meet(s.dst, span, others[o].p, others[o].n))
+                return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "dst of state %u overlaps another array of the call", i);
     }
     for (uint32_t i = 0; i < n_states; ++i)
         for (uint32_t j = 0; j < n_states; ++j) {
@@ -711,12 +673,14 @@ static needle_hip_status shape_check(uint32_t groups, uint32_t beams, uint32_t k
     return NEEDLE_HIP_OK;
 }
 
-static needle_hip_status select_check(needle_hip_ctx* c, const needle_beam_params* q, const void* logits, const uint32_t* parents,
-                                      const uint32_t* tokens, const float* scores, const uint32_t* counts) {
+static needle_hip_status select_check(needle_hip_ctx* c, const needle_beam_params* q, const void* logits, const needle_beam_state* states,
+                                      uint32_t n_states, const uint32_t* parents, const uint32_t* tokens, const float* scores,
+                                      const uint32_t* counts) {
     if (!c || !q) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "null argument");
     if (!value_known(q->value)) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "unknown value type %d", q->value);
     if (q->reserved) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "reserved is not 0");
     ST_TRY(shape_check(q->groups, q->beams, q->k));
+    if (q->vocab >= (1u << 31)) return fail(NEEDLE_HIP_ERR_UNSUPPORTED, "vocab reaches 2^31");
     if ((uint64_t)q->beams * q->vocab >= (1ull << 32)) return fail(NEEDLE_HIP_ERR_UNSUPPORTED, "beams * vocab reaches 2^32");
     if (q->groups == 0) return NEEDLE_HIP_OK;
     if (!counts || (q->k && (!parents || !tokens || !scores))) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "null output pointer");
@@ -733,12 +697,16 @@ static needle_hip_status select_check(needle_hip_ctx* c, const needle_beam_param
     if (!span_bytes(rows, q->vocab, q->row_stride, value_size(q->value), &nl) || !span_bytes(q->mask_stride ? rows : 1, words, q->mask_stride, 4, &nm))
         return fail(NEEDLE_HIP_ERR_UNSUPPORTED, "an array spans more than 2^62 bytes");
     const uint64_t np = (uint64_t)q->groups * q->k * 4;
-    const struct { const void* p; uint64_t n; } outs[4] = {{parents, np}, {tokens, np}, {scores, np}, {counts, (uint64_t)q->groups * 4}},
-        ins[4] = {{logits, nl}, {q->scores, rows * 4}, {q->finished, rows}, {q->mask, nm}};
+    const ByteRange outs[4] = {{parents, np}, {tokens, np}, {scores, np}, {counts, (uint64_t)q->groups * 4}},
+                    ins[4] = {{logits, nl}, {q->scores, rows * 4}, {q->finished, rows}, {q->mask, nm}};
     for (int i = 0; i < 4; ++i)
         for (int j = 0; j < 4; ++j)
             if (ranges_meet(outs[i].p, outs[i].n, ins[j].p, ins[j].n) || (i != j && ranges_meet(outs[i].p, outs[i].n, outs[j].p, outs[j].n)))
                 return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "an output overlaps another array");
+    if (n_states) {
+        const ByteRange all[8] = {outs[0], outs[1], outs[2], outs[3], ins[0], ins[1], ins[2], ins[3]};
+        ST_TRY(states_check(states, n_states, rows, (uint64_t)q->groups * q->k, all, 8));
+    }
     return NEEDLE_HIP_OK;
 }
 
@@ -821,10 +789,9 @@ using namespace nh;
 extern "C" needle_hip_status needle_hip_beam_select_device(needle_hip_ctx* c, const needle_beam_params* q, const void* d_logits,
                                                            const needle_beam_state* states, uint32_t n_states, uint32_t* d_out_parents,
                                                            uint32_t* d_out_tokens, float* d_out_scores, uint32_t* d_out_counts) {
-    ST_TRY(select_check(c, q, d_logits, d_out_parents, d_out_tokens, d_out_scores, d_out_counts));
+    ST_TRY(select_check(c, q, d_logits, states, n_states, d_out_parents, d_out_tokens, d_out_scores, d_out_counts));
     if (q->groups == 0) return NEEDLE_HIP_OK;
     const bool moves = n_states && q->k && q->beams;
-    if (moves) ST_TRY(states_check(states, n_states, (uint64_t)q->groups * q->beams, (uint64_t)q->groups * q->k));
     std::lock_guard g(c->mu);
     DeviceScope dev(c->device);
     HIP_TRY(dev.error());
@@ -840,7 +807,7 @@ extern "C" needle_hip_status needle_hip_beam_select(needle_hip_ctx* c, const nee
     needle_beam_params h = *q;
     h.row_stride = h.vocab;
     const uint64_t words = ((uint64_t)h.vocab + 31) / 32;
-    ST_TRY(select_check(c, &h, logits, out_parents, out_tokens, out_scores, out_counts));
+    ST_TRY(select_check(c, &h, logits, nullptr, 0, out_parents, out_tokens, out_scores, out_counts));
     if (h.mask && h.mask_stride && h.mask_stride != words) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "mask_stride is neither 0 nor a row's mask");
     if (h.groups == 0) return NEEDLE_HIP_OK;
     const size_t rows = (size_t)h.groups * h.beams, picks = (size_t)h.groups * h.k;
@@ -876,7 +843,8 @@ extern "C" needle_hip_status needle_hip_beam_reorder_device(needle_hip_ctx* c, c
         return fail(NEEDLE_HIP_ERR_UNSUPPORTED, "at most 2^31-1 beams and picks per call");
     if (groups == 0 || beams == 0 || k == 0 || n_states == 0) return NEEDLE_HIP_OK;
     if (!d_parents) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "parents is null");
-    ST_TRY(states_check(states, n_states, (uint64_t)groups * beams, (uint64_t)groups * k));
+    const ByteRange picks{d_parents, (uint64_t)groups * k * 4};
+    ST_TRY(states_check(states, n_states, (uint64_t)groups * beams, (uint64_t)groups * k, &picks, 1));
     std::lock_guard g(c->mu);
     DeviceScope dev(c->device);
     HIP_TRY(dev.error());

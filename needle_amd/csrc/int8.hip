@@ -540,9 +540,11 @@ __global__ __launch_bounds__(64 * WB * WA) void matmul_i8_tile_kernel(MatmulPara
 template <typename V, int TB, int TA, int WB, int WA, int SLOTS, bool DMA>
 static hipError_t launch_tiles_of(const MatmulParams& p, hipStream_t stream) {
     constexpr uint32_t lds = SLOTS * (TB + TA) * SLICE;
-    static const hipError_t allowed =
-        hipFuncSetAttribute((const void*)matmul_i8_tile_kernel<V, TB, TA, WB, WA, SLOTS, DMA>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (allowed != hipSuccess) return allowed;
+    if (lds >= 65536) {  // (per device, like every attribute of a kernel)
+        const hipError_t e =
+            hipFuncSetAttribute((const void*)matmul_i8_tile_kernel<V, TB, TA, WB, WA, SLOTS, DMA>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
     const uint32_t tiles_b = (uint32_t)((p.n + TB - 1) / TB), tiles_a = (p.m + TA - 1) / TA;
     hipLaunchKernelGGL((matmul_i8_tile_kernel<V, TB, TA, WB, WA, SLOTS, DMA>), dim3(tiles_b * tiles_a), dim3(64 * WB * WA), lds, stream, p, tiles_b, tiles_a);
     return hipGetLastError();
@@ -592,7 +594,7 @@ static hipError_t launch_matmul_of(const MatmulParams& p, int n_cu, hipStream_t 
         return aligned ? launch_tiles_of<V, 128, 64, 2, 2, 4, true>(p, stream) : launch_tiles_of<V, 128, 64, 2, 2, 4, false>(p, stream);
     return aligned ? launch_tiles_of<V, 64, 64, 2, 2, 4, true>(p, stream) : launch_tiles_of<V, 64, 64, 2, 2, 4, false>(p, stream);
 }
-static hipError_t launch_matmul_i8(needle_hip_ctx* c, MatmulParams p, int out_value) {
+static hipError_t launch_slab(needle_hip_ctx* c, MatmulParams p, int out_value) {
     // 1000 x 100000 x 128 to 400 MB of f32: 81 us past the cache, 103 through it; to 134 MB of bf16 (8192 x 8192 x 64) 37 and
     // 32; where rows do not start on 64 bytes (1000 x 100003) 190 and 106.
     const uint64_t size = value_size(out_value);
@@ -621,6 +623,26 @@ static hipError_t launch_matmul_i8(needle_hip_ctx* c, MatmulParams p, int out_va
     }
 }
 
+// Slabs of rows whose grids stay below 2^32 threads.
+constexpr uint64_t SLAB_N = 1ull << 26, SLAB_M = 1ull << 22;
+static hipError_t launch_matmul_i8(needle_hip_ctx* c, const MatmulParams& p, int out_value) {
+    for (uint64_t i = 0; i < p.m; i += SLAB_M)
+        for (uint64_t j = 0; j < p.n; j += SLAB_N) {
+            MatmulParams q = p;
+            q.m = (uint32_t)std::min(SLAB_M, p.m - i);
+            q.n = std::min(SLAB_N, p.n - j);
+            q.a += i * p.a_stride;
+            q.a_scales += i;
+            q.b += j * p.b_stride;
+            q.b_scales += j;
+            if (p.bias) q.bias += j;
+            q.out = (unsigned char*)p.out + (i * p.out_stride + j) * value_size(out_value);
+            const hipError_t e = launch_slab(c, q, out_value);
+            if (e != hipSuccess) return e;
+        }
+    return hipSuccess;
+}
+
 constexpr uint32_t I8_K_MAX = 131071;  // 2^14 per product at most, sums below 2^31
 
 static needle_hip_status quantize_check(needle_hip_ctx* c, const void* rows, int value, uint64_t n, uint32_t dim, uint64_t row_stride,
@@ -647,7 +669,7 @@ static needle_hip_status matmul_check(needle_hip_ctx* c, const void* a, uint32_t
     if (!c) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "ctx is null");
     if (!value_known(out_value)) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "unknown value type %d", out_value);
     if (k > I8_K_MAX) return fail(NEEDLE_HIP_ERR_UNSUPPORTED, "k = %u exceeds %u: a sum could leave 32 bits", k, I8_K_MAX);
-    if (n >= (1ull << 31)) return fail(NEEDLE_HIP_ERR_UNSUPPORTED, "at most 2^31-1 rows of b");
+    if (n >= (1ull << 31) || m >= (1u << 31)) return fail(NEEDLE_HIP_ERR_UNSUPPORTED, "at most 2^31-1 rows of a and of b");
     if (m == 0 || n == 0) return NEEDLE_HIP_OK;
     if ((!a_scales && !own_scales) || !b_scales || !out || (k > 0 && (!a || !b))) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "null argument");
     if ((m > 1 && (a_stride < k || out_stride < n)) || (n > 1 && b_stride < k))

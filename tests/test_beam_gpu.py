@@ -82,7 +82,7 @@ def _check(ctx, torch, x, scores, k, beams, normalize, mask=None, finished=None,
     there = np.isfinite(ws)
     assert np.array_equal(s[~there], ws[~there])
     # half a step of f32 for the report; the sum of exponentials in 64 bits is 1e-10 of itself off at most
-    assert (np.abs(s - ws)[there] <= 2.0 ** -24 * np.abs(ws[there]) + 1e-9).all()
+    assert (np.abs(s[there] - ws[there]) <= 2.0 ** -24 * np.abs(ws[there]) + 1e-9).all()
     return p, t, c
 
 
@@ -181,6 +181,31 @@ def test_ties_and_orders(ctx, torch, k):
         _check(ctx, torch, x[[3, 3, 3, 3]].contiguous(), s[:4], k, 2, normalize)
     _check(ctx, torch, x, s, k, 8, False)
     _check(ctx, torch, x[[0] * 40].contiguous(), np.zeros(40, np.float32), k, 40, False)
+
+
+@pytest.mark.parametrize("dtype,k", [("float32", 256), ("bfloat16", 256), ("float32", 100), ("float16", 20)])
+def test_rows_that_rise(ctx, torch, dtype, k):
+    """Logits that grow along the row, slowly to steeply: lists of every length meet chunks of which all, many or few logits
+    reach the bound, equal ones among them."""
+    rows, vocab = 1024, 20_000
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randn(rows, vocab, generator=g, device="cuda")
+    at = torch.arange(vocab, device="cuda") / 2048.0
+    slope = torch.logspace(-2.5, 1.0, rows, device="cuda")[:, None]
+    x = x + slope * at
+    x[1::4] = x[1::4].floor()                              # thousands of equal ones
+    x[2::4, 8192:9000] += 30.0                             # a block of large ones late in the row
+    x[3::4] = torch.where(torch.rand(rows // 4, vocab, generator=g, device="cuda") < 0.1, x[3::4] + 5.0, x[3::4])
+    x = x.to(getattr(torch, dtype))
+    p, t, s, c = _outputs(torch, rows, k)
+    for normalize in (True, False):
+        ctx.beam_select_device(x, None, k, p, t, s, c, beams=1, normalize=normalize)
+        want = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :k].to(torch.int32)
+        assert (c == k).all() and not p.any() and torch.equal(t, want)
+        total = torch.gather(x, 1, want.long()).double()
+        if normalize:
+            total = total - torch.logsumexp(x.double(), 1, keepdim=True)
+        assert ((s.double() - total).abs() <= 2.0 ** -24 * total.abs() + 1e-8).all()
 
 
 def test_values_over_the_range(ctx, torch):

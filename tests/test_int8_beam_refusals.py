@@ -43,7 +43,7 @@ def product(linear=False, ctx=CTX, a=at(0), a_stride=64, a_scales=at(4096), m=4,
 
 @pytest.mark.parametrize("linear", (False, True))
 @pytest.mark.parametrize("change,status", [
-    (dict(ctx=None), ARG), (dict(out_value=9), ARG), (dict(k=131072, a_stride=131072, b_stride=131072), UNSUPPORTED), (dict(n=1 << 31), UNSUPPORTED),
+    (dict(ctx=None), ARG), (dict(out_value=9), ARG), (dict(k=131072, a_stride=131072, b_stride=131072), UNSUPPORTED), (dict(n=1 << 31), UNSUPPORTED), (dict(m=1 << 31), UNSUPPORTED),
     (dict(a=None), ARG), (dict(b=None), ARG), (dict(b_scales=None), ARG), (dict(out=None), ARG), (dict(a_stride=63), ARG), (dict(b_stride=63), ARG),
     (dict(out_stride=7), ARG), (dict(out=at(32769)), ARG), (dict(bias=at(50001)), ARG), (dict(b_scales=at(16385)), ARG), (dict(out=at(0)), ARG),
     (dict(out=at(8192 + 64)), ARG), (dict(out=at(16384)), ARG), (dict(bias=at(32768)), ARG), (dict(out_stride=1 << 61), UNSUPPORTED),
@@ -68,7 +68,7 @@ def select(ctx=CTX, logits=at(0), parents=at(1 << 18), tokens=at((1 << 18) + 409
 
 @pytest.mark.parametrize("change,status", [
     (dict(ctx=None), ARG), (dict(params=False), ARG), (dict(value=4), ARG), (dict(reserved=1), ARG), (dict(k=257), UNSUPPORTED),
-    (dict(beams=1025), UNSUPPORTED), (dict(beams=1024, vocab=1 << 22, row_stride=1 << 22), UNSUPPORTED),
+    (dict(beams=1025), UNSUPPORTED), (dict(beams=1, vocab=1 << 31, row_stride=1 << 31), UNSUPPORTED), (dict(beams=1024, vocab=1 << 22, row_stride=1 << 22), UNSUPPORTED),
     (dict(groups=1 << 30, beams=2), UNSUPPORTED), (dict(groups=1 << 30, k=2, beams=1), UNSUPPORTED), (dict(logits=None), ARG), (dict(parents=None), ARG),
     (dict(tokens=None), ARG), (dict(counts=None), ARG), (dict(row_stride=99), ARG), (dict(mask=at(4096 * 9), mask_stride=3), ARG),
     (dict(finished=at(4096 * 9), end_token=100), ARG), (dict(logits=at(2)), ARG), (dict(value=2, logits=at(1)), ARG), (dict(mask=at(4096 * 9 + 2)), ARG),
@@ -102,6 +102,10 @@ def test_states(states, status):
     assert got == status if status is not None else got in (_lib.ERR_HIP, _lib.OK)  # nothing to refuse: only the device is missing
     assert reorder(state(), ctx=None) == ARG and reorder(state(), parents=None) == ARG
     assert reorder(state(), groups=0) == OK and reorder(state(), k=0) == OK
+    assert reorder(state(), parents=at((1 << 17) + 400)) == ARG
+    for other in (dict(logits=at(1 << 17)), dict(parents=at(1 << 17)), dict(scores=at((1 << 17) + 100)), dict(counts=at((1 << 17) + 700)),
+                  dict(finished=at(1 << 17)), dict(mask=at(1 << 17))):
+        assert select(states=(_lib.BeamState * 1)(_lib.BeamState(**state())), n_states=1, **other) == ARG
 
 
 def test_state_layouts():

@@ -232,6 +232,19 @@ def test_matmul_behind_four_billion(ctx, torch):
     for r, c in ((slice(0, 65), slice(0, 65)), (slice(69_900, 70_000), slice(65_900, 66_048)), (slice(65_100, 65_200), slice(30_000, 30_100))):
         _check_product(out[r, c], a[r], sa[r], b[c], sb[c], None, "bfloat16")
     del out
+    b = torch.randint(-128, 128, (2 ** 26 + 100, 16), generator=g, device="cuda", dtype=torch.int8)  # two slabs of b
+    sb = torch.rand(b.shape[0], generator=g, device="cuda")
+    out = torch.empty(2, b.shape[0], device="cuda")
+    ctx.matmul_i8_device(a[:2], sa[:2], b, sb, out, d_bias=sb)
+    for c in (slice(0, 300), slice(2 ** 26 - 150, 2 ** 26 + 100)):
+        _check_product(out[:, c], a[:2], sa[:2], b[c], sb[c], sb[c], "float32")
+    rows = torch.randint(-128, 128, (2 ** 22 + 70, 33), generator=g, device="cuda", dtype=torch.int8)  # and of a
+    sr = torch.rand(rows.shape[0], generator=g, device="cuda")
+    out = torch.empty(rows.shape[0], 5, device="cuda")
+    ctx.matmul_i8_device(rows, sr, rows[:5], sr[:5], out)
+    for r in (slice(0, 300), slice(2 ** 22 - 150, 2 ** 22 + 70)):
+        _check_product(out[r], rows[r], sr[r], rows[:5], sr[:5], None, "float32")
+    del out, rows, b
     wide = torch.randint(-127, 128, (3, 2 ** 31 + 64), generator=g, device="cuda", dtype=torch.int8)  # rows 2 GiB apart
     x = wide[:, :100]
     out = torch.empty(3, 3, device="cuda")
