@@ -302,7 +302,7 @@ __global__ __launch_bounds__(256) void matmul_i8_stream_kernel(MatmulParams p) {
         // wave w finishes the w-th share of the tiles of b
 #pragma unroll
         for (int x = 0; x < NB; ++x) {
-            if ((uint32_t)(NB == 1 ? 0 : x * 4 / NB) != wave) continue;
+            if ((uint32_t)(x * 4 / NB) != wave) continue;
 #pragma unroll
             for (int y = 0; y < NA; ++y) acc[x][y] = s_part[0][x][y][lane] + s_part[1][x][y][lane] + s_part[2][x][y][lane] + s_part[3][x][y][lane];
             finish(x);

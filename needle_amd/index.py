@@ -71,6 +71,19 @@ def _value(t, what: str) -> int:
     return v
 
 
+_torch_module = None
+
+
+def _torch():
+    """torch, for callers that hold its tensors; imported once, and only then."""
+    global _torch_module
+    if _torch_module is None:
+        import torch
+
+        _torch_module = torch
+    return _torch_module
+
+
 def _rows_of(t, name: str, dtype=None, cols=None, rows=None):
     """(rows, columns, elements from row to row) of a matrix whose rows are contiguous, any distance apart."""
     shape = t.shape
@@ -302,7 +315,7 @@ class Context:
         for t in tensors:
             if t is not None and t.get_device() != self.device:  # -1 on the host
                 raise ValueError(f"a tensor lies on {t.device}, the context on device {self.device}")
-        _wait_for_producer(tensors[0])
+        _torch().cuda.current_stream(self.device).synchronize()
 
     def quantize_rows(self, rows):
         """(codes int8 [n, dim], scales f32 [n]) of float32 or float16 host rows: symmetric, scale = max |x| * (1 / 127) per row in f32,
