@@ -184,13 +184,14 @@ struct MatmulParams {
     uint32_t past;  // the output does not fit the memory-side cache and its rows start on 64 bytes: it goes past it
 };
 
-// 16 codes of a row from place `at` on, zero from k on; nothing outside the row is read.  The last codes of a row are the
-// end of the 16 that end with it, shifted down.
+// 16 codes of a row from place `at` on, zero from k on; no word (of four bytes) without a code of the row is read.  The
+// last codes of a row are the end of the 16 that end with it, shifted down.
+template <bool ODD>
 __device__ inline u32x4 load_codes(const int8_t* row, uint32_t at, uint32_t k) {
-    if (at + 16 <= k) return *(const u32x4_any*)(row + at);
+    if (at + 16 <= k) return ODD ? load16_odd(row + at) : *(const u32x4_any*)(row + at);
     if (at >= k) return u32x4{0, 0, 0, 0};
     if (k >= 16) {
-        const u32x4 v = *(const u32x4_any*)(row + k - 16);
+        const u32x4 v = load16_odd(row + k - 16);
         const uint64_t lo = v[0] | (uint64_t)v[1] << 32, hi = v[2] | (uint64_t)v[3] << 32;
         const uint32_t bits = (at + 16 - k) * 8;  // 8 .. 120
         const uint64_t a = bits < 64 ? lo >> bits | hi << (64 - bits) : hi >> (bits - 64), b = bits < 64 ? hi >> bits : 0;
@@ -236,7 +237,7 @@ __device__ inline void store_four(typename V::bits* row, uint64_t j, uint64_t n,
 // matrix instruction's registers (16 bytes per lane, 64 codes of a row per load), those of a from the cache, the next slice
 // under way while one is multiplied.  SPLIT: the four waves of a workgroup share the rows and take every fourth slice, so
 // that a short table still has the whole chip at work; their sums meet in LDS (whole numbers: any order is exact).
-template <typename V, int NB, int NA, bool SPLIT>
+template <typename V, int NB, int NA, bool SPLIT, bool ODD>
 __global__ __launch_bounds__(256) void matmul_i8_stream_kernel(MatmulParams p) {
     constexpr uint32_t STEP = SPLIT ? 4 : 1;
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, l15 = lane & 15, quad = lane >> 4;
@@ -254,14 +255,14 @@ __global__ __launch_bounds__(256) void matmul_i8_stream_kernel(MatmulParams p) {
         const uint32_t at = s * 64;
         if (at + 64 <= p.k) {
 #pragma unroll
-            for (int x = 0; x < NB; ++x) b[x] = *(const u32x4_any*)(rb[x] + at);
+            for (int x = 0; x < NB; ++x) b[x] = ODD ? load16_odd(rb[x] + at) : *(const u32x4_any*)(rb[x] + at);
 #pragma unroll
-            for (int y = 0; y < NA; ++y) a[y] = *(const u32x4_any*)(ra[y] + at);
+            for (int y = 0; y < NA; ++y) a[y] = ODD ? load16_odd(ra[y] + at) : *(const u32x4_any*)(ra[y] + at);
         } else {
 #pragma unroll
-            for (int x = 0; x < NB; ++x) b[x] = load_codes(rb[x] - quad * 16, at + quad * 16, p.k);
+            for (int x = 0; x < NB; ++x) b[x] = load_codes<ODD>(rb[x] - quad * 16, at + quad * 16, p.k);
 #pragma unroll
-            for (int y = 0; y < NA; ++y) a[y] = load_codes(ra[y] - quad * 16, at + quad * 16, p.k);
+            for (int y = 0; y < NA; ++y) a[y] = load_codes<ODD>(ra[y] - quad * 16, at + quad * 16, p.k);
         }
     };
     auto multiply = [&](const u32x4 (&b)[NB], const u32x4 (&a)[NA]) {
@@ -375,7 +376,7 @@ __global__ __launch_bounds__(64 * WB * WA) void matmul_i8_tile_kernel(MatmulPara
             for (int i = 0; i < LOADS; ++i) held[i] = *(const u32x4_any*)(from[i] + at + chunk);
         } else {
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) held[i] = load_codes(from[i], at + chunk, p.k);
+            for (int i = 0; i < LOADS; ++i) held[i] = load_codes<false>(from[i], at + chunk, p.k);
         }
     };
     auto store = [&](uint32_t s, const u32x4 (&held)[LOADS]) {
@@ -550,18 +551,25 @@ static hipError_t launch_tiles_of(const MatmulParams& p, hipStream_t stream) {
     return hipGetLastError();
 }
 constexpr uint64_t ALIGN_MOST = 2ull << 30;  // workspace of the aligned copies; beyond it the rows pass through registers
-// Rows of k codes copied to rows of `to_stride` (a multiple of 64) with zeros behind them, a wave per row.
-__global__ __launch_bounds__(256) void align_rows_kernel(const int8_t* __restrict__ rows, uint64_t n, uint32_t k, uint64_t stride,
-                                                         int8_t* __restrict__ to, uint32_t to_stride) {
+// The rows of b and of a copied to rows of `to_stride` (a multiple of 64) with zeros behind them, a wave per row.
+__global__ __launch_bounds__(256) void align_rows_kernel(MatmulParams p, int8_t* __restrict__ to, uint32_t to_stride) {
     const uint64_t row = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= n) return;
-    for (uint32_t at = (threadIdx.x & 63) * 16; at < to_stride; at += 1024) *(u32x4*)(to + row * to_stride + at) = load_codes(rows + row * stride, at, k);
+    if (row >= p.n + p.m) return;
+    const int8_t* from = row < p.n ? p.b + row * p.b_stride : p.a + (row - p.n) * p.a_stride;
+    for (uint32_t at = (threadIdx.x & 63) * 16; at < to_stride; at += 1024) *(u32x4*)(to + row * to_stride + at) = load_codes<true>(from, at, p.k);
 }
 
+// Rows that do not all start on a multiple of four: the kernel for few rows loads them by words.  The tiles hide most of what
+// such loads cost behind their sums, and have no variant for them.
+static bool rows_odd(const MatmulParams& p) {
+    return (((uintptr_t)p.a | (uintptr_t)p.b | (p.m > 1 ? p.a_stride : 0) | (p.n > 1 ? p.b_stride : 0)) & 3) != 0;
+}
 template <typename V, int NB, int NA, bool SPLIT>
 static hipError_t launch_stream_of(const MatmulParams& p, hipStream_t stream) {
     const uint64_t tiles = (p.n + 16 * NB - 1) / (16 * NB);
-    hipLaunchKernelGGL((matmul_i8_stream_kernel<V, NB, NA, SPLIT>), dim3((uint32_t)(SPLIT ? tiles : (tiles + 3) / 4)), dim3(256), 0, stream, p);
+    const dim3 grid((uint32_t)(SPLIT ? tiles : (tiles + 3) / 4));
+    if (rows_odd(p)) hipLaunchKernelGGL((matmul_i8_stream_kernel<V, NB, NA, SPLIT, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((matmul_i8_stream_kernel<V, NB, NA, SPLIT, false>), grid, dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 static bool rows_aligned(const MatmulParams& p) {
@@ -599,22 +607,19 @@ static hipError_t launch_slab(needle_hip_ctx* c, MatmulParams p, int out_value) 
     // 32; where rows do not start on 64 bytes (1000 x 100003) 190 and 106.
     const uint64_t size = value_size(out_value);
     p.past = p.m * p.n * size > (256ull << 20) && (uintptr_t)p.out % 64 == 0 && p.out_stride * size % 64 == 0;
-    // A long product of rows that the loads cannot write to LDS themselves (odd k, strides or addresses) copies them to
-    // aligned rows first: 8192 x 8192 x 1000 of odd strides takes 104 us with the copies, 145 through registers;
-    // 8192 x 9700 x 4001 343 and 518; 300 x 66000 x 513, too few rows of a for the copy of b to pay, 69 and 46.
-    if (p.m >= 1024 && fills_big_tiles(p, c->n_cu) && !rows_aligned(p)) {
-        const uint32_t stride = (p.k + 63) / 64 * 64;
-        const uint64_t bytes = (p.n + p.m) * stride;
-        if (bytes <= ALIGN_MOST) {
-            const hipError_t e = c->scratch[5].ensure(bytes);
-            if (e != hipSuccess) return e;
-            int8_t* to = c->scratch[5].as<int8_t>();
-            hipLaunchKernelGGL(align_rows_kernel, dim3((uint32_t)((p.n + 3) / 4)), dim3(256), 0, c->stream, p.b, p.n, p.k, p.b_stride, to, stride);
-            hipLaunchKernelGGL(align_rows_kernel, dim3((p.m + 3) / 4), dim3(256), 0, c->stream, p.a, (uint64_t)p.m, p.k, p.a_stride, to + p.n * stride, stride);
-            p.b = to;
-            p.a = to + p.n * stride;
-            p.a_stride = p.b_stride = p.k = stride;
-        }
+    // A long product of rows that the loads cannot write to LDS themselves (odd k, strides or addresses): copies of them that
+    // can be (8192 x 8192 x 1000 of odd strides: 104 us with the copies, 145 through registers). Shorter products are not worth
+    // them (300 x 66000 x 513, too few rows of a for the copy of b to pay: 63 and 46; 112 x 14225 x 1971: 23 and 18).
+    const uint32_t stride = (p.k + 63) / 64 * 64;
+    const uint64_t bytes = (p.n + p.m) * stride;
+    if (p.m >= 1024 && fills_big_tiles(p, c->n_cu) && !rows_aligned(p) && bytes <= ALIGN_MOST) {
+        const hipError_t e = c->scratch[5].ensure(bytes);
+        if (e != hipSuccess) return e;
+        int8_t* to = c->scratch[5].as<int8_t>();
+        hipLaunchKernelGGL(align_rows_kernel, dim3((uint32_t)((p.n + p.m + 3) / 4)), dim3(256), 0, c->stream, p, to, stride);
+        p.b = to;
+        p.a = to + p.n * stride;
+        p.a_stride = p.b_stride = p.k = stride;
     }
     switch (out_value) {
     case NEEDLE_VALUE_F32: return launch_matmul_of<ValueF32>(p, c->n_cu, c->stream);
