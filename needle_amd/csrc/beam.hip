@@ -208,7 +208,14 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
         for (int i = 0; i < MINE; ++i) mine[i] = t + i * PIECE_THREADS < n ? s_list[t + i * PIECE_THREADS] : 0;
         if (t < 8) s_list[n + t] = 0;
         __syncthreads();
-        count_above<MINE>(s_list, n, mine, rank);
+        if (n <= PIECE_THREADS) {  // a row's short last piece, mostly: one value per thread
+            uint64_t one[1] = {mine[0]};
+            uint32_t above[1];
+            count_above<1>(s_list, n, one, above);
+            rank[0] = above[0];
+        } else {
+            count_above<MINE>(s_list, n, mine, rank);
+        }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < MINE; ++i)
@@ -348,8 +355,8 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
         }
     }
     if (n > p.len) {  // what the last bound lets through; the k largest by counting if that is still too much
-        const float b = raise();
-        const uint64_t least = (uint64_t)f2ord(fmaxf(bound, b)) << 32;
+        // (not `bound` itself: after a cut it is past the k-th's value, which stays in the list)
+        const uint64_t least = (uint64_t)f2ord(raise()) << 32;
         uint64_t mine[MINE];
 #pragma unroll
         for (int i = 0; i < MINE; ++i) mine[i] = t + i * PIECE_THREADS < n ? s_list[t + i * PIECE_THREADS] : 0;
@@ -375,8 +382,8 @@ __global__ __launch_bounds__(JOIN_THREADS) void beam_join_kernel(BeamParams p) {
     __shared__ float s_start[BEAMS_MAX];
     __shared__ uint32_t s_max[256 * GROUPS], s_n, s_bound, s_cnt[2 * JOIN_WAVES];
     __shared__ __align__(16) uint64_t s_ord[CAP + 8];
-    __shared__ uint64_t s_entry[CAP];
-    __shared__ uint16_t s_beam[CAP];
+    __shared__ __align__(16) uint64_t s_entry[CAP];
+    __shared__ __align__(16) uint16_t s_beam[CAP];
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, group = blockIdx.x;
     const size_t row0 = (size_t)group * p.beams;
     const uint64_t* list = p.list + row0 * p.pieces * p.len;
@@ -387,29 +394,36 @@ __global__ __launch_bounds__(JOIN_THREADS) void beam_join_kernel(BeamParams p) {
     };
     uint64_t head[JOIN_AT_ONCE];  // the first entries: under way while the logs are taken, and kept
     fetch(t, head);
-    for (uint32_t b = wave; b < p.beams; b += JOIN_WAVES) {
+    // As many lanes to a row as it has pieces (up to 64, a power of two): 1000 beams of one piece each took 100 us with a
+    // wave per row.
+    uint32_t lanes = 1;
+    while (lanes < 64 && lanes < p.pieces) lanes *= 2;
+    const uint32_t sub = lane & (lanes - 1);
+    for (uint32_t b = t / lanes; b < p.beams; b += JOIN_THREADS / lanes) {
         const size_t at = (row0 + b) * p.pieces;
         const float start = p.scores ? p.scores[row0 + b] : 0.0f;
         double lse = 0.0;
         if (NORMALIZE && !(p.finished && p.finished[row0 + b])) {
             float m = -__builtin_inff();
-            bool bad = false;
+            uint32_t bad = 0;
             double s = 0.0;
-            for (uint32_t i0 = 0; i0 < p.pieces; i0 += 64) {  // (a row of more than 64 pieces: its sums are scaled as its maximum grows)
-                const bool in = i0 + lane < p.pieces;
-                const float v = in ? p.peak[at + i0 + lane] : -__builtin_inff();
-                const double part = in ? p.sum[at + i0 + lane] : 0.0;
+            for (uint32_t i0 = 0; i0 < p.pieces; i0 += lanes) {  // (a row of more than 64 pieces: its sums are scaled as its maximum grows)
+                const bool in = i0 + sub < p.pieces;
+                const float v = in ? p.peak[at + i0 + sub] : -__builtin_inff();
+                const double part = in ? p.sum[at + i0 + sub] : 0.0;
                 bad |= v != v;
                 float most = fmaxf(m, v);
-                for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+                for (uint32_t o = lanes / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, (int)o));
                 if (most > -__builtin_inff()) s = (m > -__builtin_inff() ? s * exp64((double)m - (double)most) : 0.0) + (v > -__builtin_inff() ? part * exp64((double)v - (double)most) : 0.0);
                 m = most;
             }
-            bad = __any(bad) || m == __builtin_inff();
-            s = wave_sum(s);
-            lse = bad ? __longlong_as_double(0x7ff8000000000000ll) : (double)m + log(s);
+            for (uint32_t o = lanes / 2; o; o >>= 1) {
+                bad |= (uint32_t)__shfl_xor((int)bad, (int)o);
+                s += __shfl_xor(s, (int)o);
+            }
+            lse = bad || m == __builtin_inff() ? __longlong_as_double(0x7ff8000000000000ll) : (double)m + log(s);
         }
-        if (lane == 0) {
+        if (sub == 0) {
             s_lse[b] = lse;
             s_start[b] = start;
         }
@@ -501,25 +515,40 @@ __global__ __launch_bounds__(JOIN_THREADS) void beam_join_kernel(BeamParams p) {
     float* scores = p.out_scores + (size_t)group * p.k;
     if (t < 8) s_ord[n + t] = 0;
     __syncthreads();
-    for (uint32_t i = t; i < n; i += JOIN_THREADS) {
-        const uint64_t o = s_ord[i], e = s_entry[i];
-        const uint32_t b = s_beam[i];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; j += 8) {
-            uint64_t other[8];
-            bool same = false;
+    // Ranks by counting, as many threads to an entry as there are (up to 16).  Equal totals -- half-precision logits of one
+    // beam are often equal -- are told apart by beam, then by logit and token.
+    uint32_t share = 1;
+    while (share < 16 && n * share * 2 <= JOIN_THREADS) share *= 2;
+    for (uint32_t i0 = 0; i0 < n; i0 += JOIN_THREADS / share) {
+        const uint32_t i = i0 + t / share;
+        uint32_t rank = 0, b = 0;
+        uint64_t o = 0, e = 0;
+        if (i < n) {
+            o = s_ord[i];
+            e = s_entry[i];
+            b = s_beam[i];
+            for (uint32_t j = t % share * 8; j < n; j += share * 8) {
+                uint64_t other[8];
+                bool same = false;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) other[u] = s_ord[j + u];
+                for (int u = 0; u < 8; ++u) other[u] = s_ord[j + u];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                rank += other[u] > o;
-                same |= other[u] == o && j + u != i;
+                for (int u = 0; u < 8; ++u) {
+                    rank += other[u] > o;
+                    same |= other[u] == o && j + u != i;
+                }
+                if (same) {
+                    uint64_t entry[8];
+                    uint16_t beam[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) { entry[u] = s_entry[j + u]; beam[u] = s_beam[j + u]; }
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) rank += other[u] == o && (beam[u] < b || (beam[u] == b && entry[u] > e));
+                }
             }
-            if (same)  // equal totals: by beam, then by logit and token
-                for (uint32_t u = j; u < min(j + 8, n); ++u)
-                    rank += s_ord[u] == o && (s_beam[u] < b || (s_beam[u] == b && s_entry[u] > e));
         }
-        if (rank < p.k) {
+        for (uint32_t q = 1; q < share; q *= 2) rank += (uint32_t)__shfl_xor((int)rank, (int)q);
+        if (i < n && rank < p.k && t % share == 0) {
             parents[rank] = b;
             tokens[rank] = (uint32_t)~(uint32_t)e;
             scores[rank] = (float)of_order64(o);
@@ -598,10 +627,13 @@ static hipError_t launch_moves(const uint32_t* d_parents, uint32_t groups, uint3
 // ---- host side ---------------------------------------------------------------------------------
 // Bytes of a row per thread and chunk: 64 x 8 rows of 131072 bf16 logits take a third longer with 64, whose registers leave
 // room for three workgroups per CU.
-constexpr uint32_t LONG_BYTES = 32;
+constexpr uint32_t CHUNK_BYTES = 32;
 // Workgroups per CU that the pieces are cut for: the same rows take 70 us
 // with 4, 76 with 5, 73 with 8; 32 x 10 rows of 100003 f32 logits, not normalized, 30, 30 and 33.
 constexpr uint32_t PIECES_PER_CU = 4;
+// What a chunk takes a piece: 1 to 3 us, more with the logarithm and with a larger k.  10 rows of 131000 bf16 logits, k = 64,
+// take 23 us with pieces cut for it and 34 with a piece per chunk; 4 rows of 1500000 34, and 42 where it is a tenth.
+constexpr double CHUNK_NS = 2000.0;
 template <typename V, int EACH, int GROUPS>
 static void launch_pieces_of(const BeamParams& p, bool normalize, hipStream_t stream) {
     const dim3 grid(p.rows * p.pieces), block(PIECE_THREADS);
@@ -611,16 +643,10 @@ static void launch_pieces_of(const BeamParams& p, bool normalize, hipStream_t st
     else hipLaunchKernelGGL((beam_piece_kernel<V, EACH, GROUPS, false, false>), grid, block, 0, stream, p);
 }
 template <typename V>
-static void launch_pieces(const BeamParams& p, bool normalize, bool short_chunks, hipStream_t stream) {
+static void launch_pieces(const BeamParams& p, bool normalize, hipStream_t stream) {
     // 256 maxima tell the k <= 64 largest of a chunk well enough (about 1.2 k logits reach the bound), more need 1024
-    if (short_chunks) {
-        if (p.k <= 64) launch_pieces_of<V, 8, 1>(p, normalize, stream);
-        else launch_pieces_of<V, 8, 4>(p, normalize, stream);
-    } else if (p.k <= 64) {
-        launch_pieces_of<V, (int)LONG_BYTES / V::size, 1>(p, normalize, stream);
-    } else {
-        launch_pieces_of<V, (int)LONG_BYTES / V::size, 4>(p, normalize, stream);
-    }
+    if (p.k <= 64) launch_pieces_of<V, (int)CHUNK_BYTES / V::size, 1>(p, normalize, stream);
+    else launch_pieces_of<V, (int)CHUNK_BYTES / V::size, 4>(p, normalize, stream);
 }
 
 struct ByteRange { const void* p; uint64_t n; };
@@ -730,20 +756,16 @@ static needle_hip_status select_enqueue(needle_hip_ctx* c, const needle_beam_par
     BeamParams p{};
     p.beams = q.beams; p.vocab = q.vocab; p.k = q.k; p.end_token = q.end_token;
     p.row_stride = q.row_stride; p.mask_stride = q.mask_stride;
-    // Few rows: chunks of 2048 logits, a workgroup each, so that more of the chip works on a row.  Otherwise chunks of
-    // LONG_BYTES per thread, and as many pieces as give the chip about PIECES_PER_CU workgroups per CU.
-    const uint64_t all_rows = (uint64_t)q.groups * q.beams;
-    const uint64_t long_chunk = PIECE_THREADS * LONG_BYTES / value_size(q.value), long_chunks = (q.vocab + long_chunk - 1) / long_chunk;
-    const bool short_chunks = all_rows * long_chunks < 2ull * c->n_cu;
-    if (short_chunks) {
-        p.chunks_per_piece = 1;
-        p.pieces = (q.vocab + 2047) / 2048;
-    } else {
-        const uint64_t want = std::min<uint64_t>(long_chunks, std::max<uint64_t>(1, ((uint64_t)PIECES_PER_CU * c->n_cu + all_rows - 1) / all_rows));
-        p.chunks_per_piece = (uint32_t)((long_chunks + want - 1) / want);
-        p.pieces = (uint32_t)((long_chunks + p.chunks_per_piece - 1) / p.chunks_per_piece);
-    }
-    p.len = std::max<uint32_t>(2 * q.k, 32);  // room for what the last bound lets through, so that few lists need an exact cut
+    p.len = std::max<uint32_t>(q.k + q.k / 2, 16);  // room for what the last bound lets through, so that few lists need an exact cut
+    // As many pieces as give the chip PIECES_PER_CU workgroups per CU; but a group's lists meet in one workgroup, which takes
+    // them at once up to JOIN_AT_ONCE entries per thread and then 0.5 ns per entry, while a chunk takes a piece CHUNK_NS: the
+    // count where the two add up to least.
+    const uint64_t all_rows = (uint64_t)q.groups * q.beams, chunk = PIECE_THREADS * CHUNK_BYTES / value_size(q.value), chunks = (q.vocab + chunk - 1) / chunk;
+    const uint64_t share = ((uint64_t)PIECES_PER_CU * c->n_cu + all_rows - 1) / all_rows, entries = (uint64_t)q.beams * p.len;
+    const uint64_t joined = std::max<uint64_t>(JOIN_THREADS * JOIN_AT_ONCE / entries, (uint64_t)std::sqrt((double)chunks * CHUNK_NS / (0.5 * (double)entries)));
+    const uint64_t want = std::max<uint64_t>(1, std::min(chunks, std::min(share, joined)));
+    p.chunks_per_piece = (uint32_t)((chunks + want - 1) / want);
+    p.pieces = (uint32_t)((chunks + p.chunks_per_piece - 1) / p.chunks_per_piece);
     {
         const uint32_t d = p.pieces * p.len;  // rounded up 32-bit reciprocal: exact for numerators below 2^31
         while ((1ull << p.per_row_shift) < d) ++p.per_row_shift;
@@ -767,9 +789,9 @@ static needle_hip_status select_enqueue(needle_hip_ctx* c, const needle_beam_par
         p.mask = q.mask ? q.mask + r0 * q.mask_stride : nullptr;
         p.out_parents = parents + g0 * q.k; p.out_tokens = tokens + g0 * q.k; p.out_scores = scores + g0 * q.k; p.out_counts = counts + g0;
         switch (q.value) {
-        case NEEDLE_VALUE_F32: launch_pieces<ValueF32>(p, normalize, short_chunks, c->stream); break;
-        case NEEDLE_VALUE_F16: launch_pieces<ValueF16>(p, normalize, short_chunks, c->stream); break;
-        default: launch_pieces<ValueBF16>(p, normalize, short_chunks, c->stream);
+        case NEEDLE_VALUE_F32: launch_pieces<ValueF32>(p, normalize, c->stream); break;
+        case NEEDLE_VALUE_F16: launch_pieces<ValueF16>(p, normalize, c->stream); break;
+        default: launch_pieces<ValueBF16>(p, normalize, c->stream);
         }
         HIP_TRY(hipGetLastError());
         const dim3 grid(p.groups), block(JOIN_THREADS);

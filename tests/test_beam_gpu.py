@@ -107,6 +107,22 @@ def test_select(ctx, torch, dtype, groups, beams, vocab, k):
         _check(ctx, torch, x, _scores(vocab, rows), k, beams, normalize)
 
 
+@pytest.mark.parametrize("groups,beams,vocab,k,dtype", [(1, 1000, 300, 5, "float32"), (2, 100, 20_000, 7, "float32"), (3, 33, 9000, 64, "float16"),
+                                                        (1, 10, 40_000, 64, "bfloat16"), (1, 7, 70_000, 33, "float16"), (1, 3, 20_000, 256, "bfloat16")])
+def test_lists_that_meet_in_one_group(ctx, torch, groups, beams, vocab, k, dtype):
+    """Many beams, or many pieces of long lists, with rows among them that end, offer nothing or have no sum."""
+    rows = groups * beams
+    x = _logits(torch, beams, rows, vocab, dtype)
+    finished = np.zeros(rows, np.uint8)
+    finished[::5] = 1
+    x[1] = -INF
+    x[2::9, vocab - 1] = float("nan")
+    scores = _scores(k, rows)
+    for normalize in (True, False):
+        _check(ctx, torch, x, scores, k, beams, normalize, finished=finished, end=vocab - 1)
+        _check(ctx, torch, x, None, k, beams, normalize)
+
+
 @pytest.mark.parametrize("dtype,vocab,pad", [("float32", 1001, 3), ("bfloat16", 9000, 1), ("float16", 8200, 5)])
 def test_rows_that_lie_apart(ctx, torch, dtype, vocab, pad):
     x = _logits(torch, 4, 12, vocab, dtype, pad)
