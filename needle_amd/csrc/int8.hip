@@ -28,10 +28,11 @@ __device__ inline int code_of(float x, float s, float inv) {
 constexpr float PER_STEP = 1.0f / 127.0f;  // the f32 nearest to it
 constexpr float TINY_ROW = 0x1p-60f, TINY_UP = 0x1p80f;
 
-// LANES lanes of a wave hold a row in registers, PER vectors of WIDE values each, so that it is read once: 16 bytes per lane
-// and load, from any address, WIDE codes per store.  Rows longer than 64 * PER * WIDE values are read twice (the second
-// time from the cache) by a workgroup.  The bytes bound it: 200003 x 384 f32 take 68 us, 5.6 TB/s (a wave per row, a value per
-// load, read twice: 174 us); 16384 x 4096 bf16 45 us, 4.4 TB/s.
+// LANES lanes (256: the four waves of a workgroup) hold a row in registers, PER vectors of WIDE values each, so that it is
+// read once: 16 bytes per lane and load, from any address, WIDE codes per store.  Rows longer than 256 * 8 * WIDE values are
+// read twice (the second time from the cache) by a workgroup of 1024.  The bytes bound it: 200003 x 384 f32 take 68 us, 5.6
+// TB/s (a wave per row, a value per load, read twice: 174 us); 16384 x 4096 f32 56 us, 6.0 TB/s (read twice by 1024 threads:
+// 5164 x 3153 31 us, so 16 now).
 template <typename V, int LANES, int PER>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename V::bits* __restrict__ x, uint64_t n, uint32_t dim,
                                                             uint64_t x_stride, int8_t* __restrict__ codes, uint64_t c_stride,
@@ -63,7 +64,13 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename V::bi
         }
     }
 #pragma unroll
-    for (int o = LANES / 2; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    for (int o = LANES < 64 ? LANES / 2 : 32; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    if (LANES == 256) {
+        __shared__ uint32_t s_top[4];
+        if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
+        __syncthreads();
+        top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+    }
     const float big = __uint_as_float(top), s = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : big * PER_STEP;
     if (lane == 0) scales[row] = s;
     const bool some = s > 0.0f;
@@ -149,14 +156,21 @@ template <typename V>
 static hipError_t launch_quantize_rows_of(const typename V::bits* x, uint64_t n, uint32_t dim, uint64_t x_stride, int8_t* codes, uint64_t c_stride,
                                           float* scales, hipStream_t stream) {
     const uint32_t loads = (dim + 16 / V::size - 1) / (16 / V::size);  // of a row
-    if (loads <= 8) launch_quantize_of<V, 8, 1>(x, n, dim, x_stride, codes, c_stride, scales, stream);
-    else if (loads <= 16) launch_quantize_of<V, 16, 1>(x, n, dim, x_stride, codes, c_stride, scales, stream);
+    // several loads per lane where the row has them, few idle lanes: us of 1000000 x 64 f32 with <4, 2>, <8, 1>: 56, 69 (less a
+    // call's 17); 100000 x 384 f16 with <16, 3>, <32, 2>: 24, 34; 3000000 x 24 bf16 with <4, 1>, <8, 1>: 64, 128; 16384 x 4096
+    // bf16 with <256, 2>, <64, 8>: 41, 44; 30000 x 1000 f32 with <64, 4>, <256, 1>: 23, 30
+    if (loads <= 4) launch_quantize_of<V, 4, 1>(x, n, dim, x_stride, codes, c_stride, scales, stream);
+    else if (loads <= 8) launch_quantize_of<V, 4, 2>(x, n, dim, x_stride, codes, c_stride, scales, stream);
+    else if (loads <= 16) launch_quantize_of<V, 8, 2>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else if (loads <= 32) launch_quantize_of<V, 16, 2>(x, n, dim, x_stride, codes, c_stride, scales, stream);
+    else if (loads <= 48) launch_quantize_of<V, 16, 3>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else if (loads <= 64) launch_quantize_of<V, 32, 2>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else if (loads <= 96) launch_quantize_of<V, 32, 3>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else if (loads <= 128) launch_quantize_of<V, 64, 2>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else if (loads <= 256) launch_quantize_of<V, 64, 4>(x, n, dim, x_stride, codes, c_stride, scales, stream);
-    else if (loads <= 512) launch_quantize_of<V, 64, 8>(x, n, dim, x_stride, codes, c_stride, scales, stream);
+    else if (loads <= 512) launch_quantize_of<V, 256, 2>(x, n, dim, x_stride, codes, c_stride, scales, stream);
+    else if (loads <= 1024) launch_quantize_of<V, 256, 4>(x, n, dim, x_stride, codes, c_stride, scales, stream);
+    else if (loads <= 2048) launch_quantize_of<V, 256, 8>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else hipLaunchKernelGGL((quantize_long_rows_kernel<V>), dim3((uint32_t)std::min<uint64_t>(n, 1u << 16)), dim3(1024), 0, stream, x, n, dim, x_stride, codes, c_stride, scales);
     return hipGetLastError();
 }
@@ -607,12 +621,13 @@ static hipError_t launch_slab(needle_hip_ctx* c, MatmulParams p, int out_value) 
     // 32; where rows do not start on 64 bytes (1000 x 100003) 190 and 106.
     const uint64_t size = value_size(out_value);
     p.past = p.m * p.n * size > (256ull << 20) && (uintptr_t)p.out % 64 == 0 && p.out_stride * size % 64 == 0;
-    // A long product of rows that the loads cannot write to LDS themselves (odd k, strides or addresses): copies of them that
-    // can be (8192 x 8192 x 1000 of odd strides: 104 us with the copies, 145 through registers). Shorter products are not worth
-    // them (300 x 66000 x 513, too few rows of a for the copy of b to pay: 63 and 46; 112 x 14225 x 1971: 23 and 18).
+    // Rows that the loads cannot write to LDS themselves (odd k, strides or addresses): a product of more tiles than CUs copies
+    // them to rows that can be first, where enough sums are made of each code.  us of the copies and the product, and of the
+    // product through registers: 8192 x 8192 x 1000 104, 145; 2256 x 6573 x 1946 62, 83; 4196 x 5755 x 218 28, 34; 600 x 60000 x
+    // 513 62, 64; not so 300 x 66000 x 513 63, 46; 2000 x 2000 x 301 11, 7.
     const uint32_t stride = (p.k + 63) / 64 * 64;
-    const uint64_t bytes = (p.n + p.m) * stride;
-    if (p.m >= 1024 && fills_big_tiles(p, c->n_cu) && !rows_aligned(p) && bytes <= ALIGN_MOST) {
+    const uint64_t bytes = (p.n + p.m) * stride, tiles = ((p.n + 127) / 128) * ((p.m + 127) / 128);
+    if (!rows_aligned(p) && tiles > (uint64_t)c->n_cu && p.m * p.n >= 512 * (p.m + p.n) && bytes <= ALIGN_MOST) {
         const hipError_t e = c->scratch[5].ensure(bytes);
         if (e != hipSuccess) return e;
         int8_t* to = c->scratch[5].as<int8_t>();

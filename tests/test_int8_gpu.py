@@ -55,7 +55,8 @@ def _quantize(torch, ctx, t, codes=None):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,dim", [(1, 1), (7, 3), (5, 16), (3, 63), (130, 64), (2, 129), (33, 384), (9, 768), (6, 1000), (3, 1024), (2, 1025),
-                                   (5, 4096), (2, 5000), (1, 20011), (1001, 24)])
+                                   (5, 4096), (2, 5000), (1, 20011), (1001, 24), (70, 9), (65, 31), (9, 190), (5, 2049), (4, 4095), (3, 8191),
+                                   (3, 8193), (2, 16_384), (2, 16_385)])
 def test_quantize_rows(ctx, torch, dtype, n, dim):
     rng = np.random.default_rng(n * 31 + dim)
     t = torch.from_numpy(_rows(rng, n, dim)).to("cuda").to(getattr(torch, dtype))
