@@ -149,6 +149,7 @@ extern "C" void needle_hip_shutdown(needle_hip_ctx* c) {
     if (c->stream) (void)hipStreamSynchronize(c->stream);
     destroy_side_stream(c);
     for (auto& b : c->scratch) b.release();
+    if (c->done) (void)hipHostFree(c->done);
     for (int i = 0; i < 4; ++i)
         if (c->ev[i]) (void)hipEventDestroy(c->ev[i]);
     if (c->stream) (void)hipStreamDestroy(c->stream);

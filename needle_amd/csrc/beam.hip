@@ -819,7 +819,7 @@ extern "C" needle_hip_status needle_hip_beam_select_device(needle_hip_ctx* c, co
     HIP_TRY(dev.error());
     ST_TRY(select_enqueue(c, *q, d_logits, d_out_parents, d_out_tokens, d_out_scores, d_out_counts));
     if (moves) HIP_TRY(launch_moves(d_out_parents, q->groups, q->beams, q->k, states, n_states, c->n_cu, c->stream));
-    HIP_TRY(hipStreamSynchronize(c->stream));
+    HIP_TRY(wait_done(c));
     return NEEDLE_HIP_OK;
 }
 
@@ -871,6 +871,6 @@ extern "C" needle_hip_status needle_hip_beam_reorder_device(needle_hip_ctx* c, c
     DeviceScope dev(c->device);
     HIP_TRY(dev.error());
     HIP_TRY(launch_moves(d_parents, groups, beams, k, states, n_states, c->n_cu, c->stream));
-    HIP_TRY(hipStreamSynchronize(c->stream));
+    HIP_TRY(wait_done(c));
     return NEEDLE_HIP_OK;
 }

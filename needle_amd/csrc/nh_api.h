@@ -110,6 +110,8 @@ struct needle_hip_ctx {
     std::recursive_mutex mu;  // recursive: a host-pointer operator holds it across staging, its _device form and the copy back
     std::mutex prof_mu;  // held by a whole search while profiling is on (the events ev[] are shared by the context's indexes)
     nh::DevBuf scratch[8];  // operator-level calls
+    uint32_t* done = nullptr;      // pinned word that wait_done's kernel counts up (int8.hip)
+    uint32_t done_count = 0;
     void* topk_static = nullptr;   // device address of the static top-k workspace on this context's device (ops.hip)
     size_t topk_static_bytes = 0;
 };

@@ -85,4 +85,7 @@ inline bool ranges_meet(const void* a, uint64_t na, const void* b, uint64_t nb) 
     return a && b && na && nb && x < y + nb && y < x + na;
 }
 
+// Waits until everything on the context's stream has finished; the caller holds the context's lock.
+hipError_t wait_done(needle_hip_ctx* c);
+
 }  // namespace nh

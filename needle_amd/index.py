@@ -84,6 +84,22 @@ def _torch():
     return _torch_module
 
 
+_stream_of = None  # (current device, current stream of a device, wait for a stream) where torch has the raw handles
+
+
+def _wait_for_stream(device: int) -> None:
+    """torch's current stream on `device` has finished: what its synchronize() does, in a third of the time where torch tells
+    the handle.  Stream 0 names no device, so this holds on the current device only."""
+    global _stream_of
+    if _stream_of is None:
+        inner = _torch()._C
+        names = [getattr(inner, name, None) for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream")]
+        wait = C.CFUNCTYPE(C.c_int, C.c_void_p)(("hipStreamSynchronize", _lib.lib()))
+        _stream_of = (*names, wait) if all(names) else ()
+    if not _stream_of or _stream_of[0]() != device or _stream_of[2](_stream_of[1](device)):
+        _torch().cuda.current_stream(device).synchronize()  # (raises what the runtime reports)
+
+
 def _rows_of(t, name: str, dtype=None, cols=None, rows=None):
     """(rows, columns, elements from row to row) of a matrix whose rows are contiguous, any distance apart."""
     shape = t.shape
@@ -315,7 +331,7 @@ class Context:
         for t in tensors:
             if t is not None and t.get_device() != self.device:  # -1 on the host
                 raise ValueError(f"a tensor lies on {t.device}, the context on device {self.device}")
-        _torch().cuda.current_stream(self.device).synchronize()
+        _wait_for_stream(self.device)
 
     def quantize_rows(self, rows):
         """(codes int8 [n, dim], scales f32 [n]) of float32 or float16 host rows: symmetric, scale = max |x| * (1 / 127) per row in f32,

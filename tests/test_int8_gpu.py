@@ -322,3 +322,49 @@ def test_calls_from_threads_and_streams(ctx, torch):
         ctx.linear_i8_device(x, b, sb, out)
         for r in range(6):
             assert torch.equal(got[i][r], out)
+
+
+def test_outputs_are_there_when_a_call_returns(ctx, torch):
+    """Every call's output read at once, on another stream than any the call or its inputs used, and copied to the host."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    other = torch.cuda.Stream()
+    for i in range(300):
+        n, dim = (1, 7, 300, 20_000)[i % 4], (64, 333, 1024)[i % 3]
+        x = torch.randn(n, dim, generator=g, device="cuda")
+        codes, scales = torch.full((n, dim), 99, dtype=torch.int8, device="cuda"), torch.full((n,), -1.0, device="cuda")
+        want = x.abs().amax(1) * torch.tensor(1.0 / 127.0, device="cuda")
+        torch.cuda.synchronize()
+        ctx.quantize_rows_device(x, codes, scales)
+        with torch.cuda.stream(other):
+            here = codes.clone(), scales.clone()
+        there = scales.cpu()
+        other.synchronize()
+        assert torch.equal(here[1], want) and torch.equal(there, want.cpu())
+        assert (here[0].abs().amax(1) == 127).all()
+
+
+def test_inputs_under_way_on_another_stream(ctx, torch):
+    """A call waits for torch's current stream, whichever that is."""
+    side = torch.cuda.Stream()
+    big = torch.randn(8192, 8192, device="cuda")
+    for stream in (side, torch.cuda.default_stream()):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            x = (big @ big)[:64].contiguous()
+            codes, scales = torch.empty(64, 8192, dtype=torch.int8, device="cuda"), torch.empty(64, device="cuda")
+            ctx.quantize_rows_device(x, codes, scales)
+            want = x.abs().amax(1) * torch.tensor(1.0 / 127.0, device="cuda")
+            assert torch.equal(scales, want)
+
+
+def test_a_call_of_milliseconds(ctx, torch):
+    g = torch.Generator(device="cuda").manual_seed(4)
+    m, n, k = 8192, 65_536, 4096
+    a, b = (torch.randint(-127, 128, (r, k), generator=g, device="cuda", dtype=torch.int8) for r in (m, n))
+    sa, sb = torch.ones(m, device="cuda"), torch.ones(n, device="cuda")
+    out = torch.full((m, n), float("nan"), device="cuda")
+    ctx.matmul_i8_device(a, sa, b, sb, out)
+    assert not out.isnan().any()
+    at, bt = torch.randint(0, m, (500,), device="cuda"), torch.randint(0, n, (500,), device="cuda")
+    want = (a[at].double() * b[bt].double()).sum(1)  # below 2^27: a whole number, rounded once
+    assert torch.equal(out[at, bt], want.float())
