@@ -373,11 +373,13 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
 }
 
 // One group: the logs of its rows' sums, the totals of what the pieces listed, and the k best of them.  A thread fetches
-// eight entries at a time: one workgroup serves a group, so what counts is that no load waits for the one before it.
-constexpr uint32_t JOIN_THREADS = 1024, JOIN_WAVES = JOIN_THREADS / 64, JOIN_AT_ONCE = 8;
-template <int GROUPS, bool NORMALIZE>
+// AT_ONCE entries at a time.  A chain of short steps by one workgroup: what bounds it are latencies, those of the first
+// fetch of each instruction among them, so that less code is faster: 4 beams of 32000 f32 logits take 5.5 us with AT_ONCE 2,
+// 6.8 with 8 (and 6.8 with 256 threads and 8); 10240 entries 8.3 with 4, 8.9 with 8.
+constexpr uint32_t JOIN_THREADS = 1024, JOIN_AT_ONCE = 4, JOIN_FEW = 2;
+template <uint32_t AT_ONCE, int GROUPS, bool NORMALIZE>
 __global__ __launch_bounds__(JOIN_THREADS) void beam_join_kernel(BeamParams p) {
-    constexpr uint32_t CAP = 2048;
+    constexpr uint32_t CAP = 2048, JOIN_WAVES = JOIN_THREADS / 64;
     __shared__ double s_lse[BEAMS_MAX];
     __shared__ float s_start[BEAMS_MAX];
     __shared__ uint32_t s_max[256 * GROUPS], s_n, s_bound, s_cnt[2 * JOIN_WAVES];
@@ -388,11 +390,11 @@ __global__ __launch_bounds__(JOIN_THREADS) void beam_join_kernel(BeamParams p) {
     const size_t row0 = (size_t)group * p.beams;
     const uint64_t* list = p.list + row0 * p.pieces * p.len;
     const uint32_t slots = p.beams * p.pieces * p.len;  // below 2^31
-    auto fetch = [&](uint32_t i0, uint64_t (&e)[JOIN_AT_ONCE]) {
+    auto fetch = [&](uint32_t i0, uint64_t (&e)[AT_ONCE]) {
 #pragma unroll
-        for (uint32_t u = 0; u < JOIN_AT_ONCE; ++u) e[u] = i0 + u * JOIN_THREADS < slots ? list[i0 + u * JOIN_THREADS] : 0;
+        for (uint32_t u = 0; u < AT_ONCE; ++u) e[u] = i0 + u * JOIN_THREADS < slots ? list[i0 + u * JOIN_THREADS] : 0;
     };
-    uint64_t head[JOIN_AT_ONCE];  // the first entries: under way while the logs are taken, and kept
+    uint64_t head[AT_ONCE];  // the first entries: under way while the logs are taken, and kept
     fetch(t, head);
     // As many lanes to a row as it has pieces (up to 64, a power of two): 1000 beams of one piece each took 100 us with a
     // wave per row.
@@ -429,7 +431,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void beam_join_kernel(BeamParams p) {
         }
     }
     if (t == 0) s_n = 0;
-    if (t < 256 * GROUPS) s_max[t] = 0;
+    for (uint32_t i = t; i < 256 * GROUPS; i += JOIN_THREADS) s_max[i] = 0;
     __syncthreads();
     // order of the total and beam of a list entry; an ended beam's entry holds a logit of 0 and no sum
     auto total_of = [&](uint64_t e, uint32_t i, uint32_t* beam) -> uint64_t {
@@ -439,11 +441,11 @@ __global__ __launch_bounds__(JOIN_THREADS) void beam_join_kernel(BeamParams p) {
     };
     // f(order, entry, beam, slot) for every slot that holds an entry of a total
     auto each = [&](auto f) {
-        for (uint32_t i0 = t; i0 < slots; i0 += JOIN_THREADS * JOIN_AT_ONCE) {
-            uint64_t e[JOIN_AT_ONCE];
+        for (uint32_t i0 = t; i0 < slots; i0 += JOIN_THREADS * AT_ONCE) {
+            uint64_t e[AT_ONCE];
             if (i0 != t) fetch(i0, e);
 #pragma unroll
-            for (uint32_t u = 0; u < JOIN_AT_ONCE; ++u) {
+            for (uint32_t u = 0; u < AT_ONCE; ++u) {
                 const uint64_t entry = i0 == t ? head[u] : e[u];
                 uint32_t beam = 0;
                 const uint64_t o = entry ? total_of(entry, i0 + u * JOIN_THREADS, &beam) : 0;
@@ -634,6 +636,7 @@ constexpr uint32_t PIECES_PER_CU = 4;
 // What a chunk takes a piece: 1 to 3 us, more with the logarithm and with a larger k.  10 rows of 131000 bf16 logits, k = 64,
 // take 23 us with pieces cut for it and 34 with a piece per chunk; 4 rows of 1500000 34, and 42 where it is a tenth.
 constexpr double CHUNK_NS = 2000.0;
+constexpr uint32_t JOIN_ENTRIES = 8192;
 template <typename V, int EACH, int GROUPS>
 static void launch_pieces_of(const BeamParams& p, bool normalize, hipStream_t stream) {
     const dim3 grid(p.rows * p.pieces), block(PIECE_THREADS);
@@ -647,6 +650,17 @@ static void launch_pieces(const BeamParams& p, bool normalize, hipStream_t strea
     // 256 maxima tell the k <= 64 largest of a chunk well enough (about 1.2 k logits reach the bound), more need 1024
     if (p.k <= 64) launch_pieces_of<V, (int)CHUNK_BYTES / V::size, 1>(p, normalize, stream);
     else launch_pieces_of<V, (int)CHUNK_BYTES / V::size, 4>(p, normalize, stream);
+}
+
+template <uint32_t AT_ONCE, int GROUPS>
+static void launch_join_of(const BeamParams& p, bool normalize, hipStream_t stream) {
+    if (normalize) hipLaunchKernelGGL((beam_join_kernel<AT_ONCE, GROUPS, true>), dim3(p.groups), dim3(JOIN_THREADS), 0, stream, p);
+    else hipLaunchKernelGGL((beam_join_kernel<AT_ONCE, GROUPS, false>), dim3(p.groups), dim3(JOIN_THREADS), 0, stream, p);
+}
+static void launch_join(const BeamParams& p, bool normalize, hipStream_t stream) {
+    if (p.k > 64) launch_join_of<JOIN_AT_ONCE, 4>(p, normalize, stream);
+    else if (p.beams * p.pieces * p.len > JOIN_FEW * JOIN_THREADS) launch_join_of<JOIN_AT_ONCE, 1>(p, normalize, stream);
+    else launch_join_of<JOIN_FEW, 1>(p, normalize, stream);
 }
 
 struct ByteRange { const void* p; uint64_t n; };
@@ -758,11 +772,11 @@ static needle_hip_status select_enqueue(needle_hip_ctx* c, const needle_beam_par
     p.row_stride = q.row_stride; p.mask_stride = q.mask_stride;
     p.len = std::max<uint32_t>(q.k + q.k / 2, 16);  // room for what the last bound lets through, so that few lists need an exact cut
     // As many pieces as give the chip PIECES_PER_CU workgroups per CU; but a group's lists meet in one workgroup, which takes
-    // them at once up to JOIN_AT_ONCE entries per thread and then 0.5 ns per entry, while a chunk takes a piece CHUNK_NS: the
-    // count where the two add up to least.
+    // 3 us longer for JOIN_ENTRIES of them than for a few and then 0.5 ns per entry, while a chunk takes a piece CHUNK_NS:
+    // the count where the two add up to least.
     const uint64_t all_rows = (uint64_t)q.groups * q.beams, chunk = PIECE_THREADS * CHUNK_BYTES / value_size(q.value), chunks = (q.vocab + chunk - 1) / chunk;
     const uint64_t share = ((uint64_t)PIECES_PER_CU * c->n_cu + all_rows - 1) / all_rows, entries = (uint64_t)q.beams * p.len;
-    const uint64_t joined = std::max<uint64_t>(JOIN_THREADS * JOIN_AT_ONCE / entries, (uint64_t)std::sqrt((double)chunks * CHUNK_NS / (0.5 * (double)entries)));
+    const uint64_t joined = std::max<uint64_t>(JOIN_ENTRIES / entries, (uint64_t)std::sqrt((double)chunks * CHUNK_NS / (0.5 * (double)entries)));
     const uint64_t want = std::max<uint64_t>(1, std::min(chunks, std::min(share, joined)));
     p.chunks_per_piece = (uint32_t)((chunks + want - 1) / want);
     p.pieces = (uint32_t)((chunks + p.chunks_per_piece - 1) / p.chunks_per_piece);
@@ -794,11 +808,7 @@ static needle_hip_status select_enqueue(needle_hip_ctx* c, const needle_beam_par
         default: launch_pieces<ValueBF16>(p, normalize, c->stream);
         }
         HIP_TRY(hipGetLastError());
-        const dim3 grid(p.groups), block(JOIN_THREADS);
-        if (q.k <= 64 && normalize) hipLaunchKernelGGL((beam_join_kernel<1, true>), grid, block, 0, c->stream, p);
-        else if (q.k <= 64) hipLaunchKernelGGL((beam_join_kernel<1, false>), grid, block, 0, c->stream, p);
-        else if (normalize) hipLaunchKernelGGL((beam_join_kernel<4, true>), grid, block, 0, c->stream, p);
-        else hipLaunchKernelGGL((beam_join_kernel<4, false>), grid, block, 0, c->stream, p);
+        launch_join(p, normalize, c->stream);
         HIP_TRY(hipGetLastError());
     }
     return NEEDLE_HIP_OK;
