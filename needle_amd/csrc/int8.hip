@@ -32,62 +32,84 @@ constexpr float TINY_ROW = 0x1p-60f, TINY_UP = 0x1p80f;
 // LANES lanes (256: the four waves of a workgroup) hold a row in registers, PER vectors of WIDE values each, so that it is
 // read once: 16 bytes per lane and load, from any address, WIDE codes per store.  Rows longer than 256 * 8 * WIDE values are
 // read twice (the second time from the cache) by a workgroup of 1024.  The bytes bound it: 200003 x 384 f32 take 68 us, 5.6
-// TB/s (a wave per row, a value per load, read twice: 174 us); 16384 x 4096 f32 56 us, 6.0 TB/s (read twice by 1024 threads:
-// 5164 x 3153 31 us, so 16 now).
+// TB/s (a wave per row, a value per load, read twice: 174 us); 41593 x 1505 bf16 35 us, 5.4 TB/s (with every residue taken, a
+// dozen instructions more per value, 54).
+//
+// Of a row that is neither tiny nor NaN most codes need no residue: x / s and x * (1 / s) differ by 127 * 2^-24 at most, so
+// where the latter lies further than that from a half, its nearest whole number is the code.  Adding 1.5 * 2^23 to the
+// product leaves that number in the low bits of the sum.  A wave that meets a half takes the residues of that load.
 template <typename V, int LANES, int PER>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename V::bits* __restrict__ x, uint64_t n, uint32_t dim,
                                                             uint64_t x_stride, int8_t* __restrict__ codes, uint64_t c_stride,
                                                             float* __restrict__ scales) {
     constexpr int WIDE = 16 / V::size;
-    typedef int8_t codes_t __attribute__((ext_vector_type(WIDE), aligned(1)));
+    constexpr float WHOLE = 12582912.0f, HALF = 0.49998f;
+    typedef uint32_t codes_t __attribute__((ext_vector_type(WIDE / 4), aligned(1)));
+    typedef typename V::bits bits_t __attribute__((ext_vector_type(WIDE)));
     const uint32_t lane = threadIdx.x % LANES;
-    const uint64_t row = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
-    if (row >= n) return;
+    const uint64_t at = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
+    if (LANES <= 64 && at >= n) return;
+    const uint64_t row = LANES <= 64 ? at : min(at, n - 1);  // (two rows of 128 lanes share a barrier: the last one twice if need be)
     const typename V::bits* p = x + row * x_stride;
     int8_t* c = codes + row * c_stride;
-    float v[PER][WIDE];
-    uint32_t top = 0;  // |x| as bits: ordered like the values, NaN and infinity on top
+    bits_t v[PER];
+    bits_t tops = 0;  // |x| as bits: ordered like the values, NaN and infinity on top
+    auto load = [&](uint32_t j) {
+        bits_t one;
+        if (j + WIDE <= dim) return __builtin_bit_cast(bits_t, *(const u32x4_any*)(p + j));
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const uint32_t j = (i * LANES + lane) * WIDE;
-        typename V::bits one[WIDE];
-        if (j + WIDE <= dim) {
-            const u32x4 raw = *(const u32x4_any*)(p + j);
-            __builtin_memcpy(one, &raw, 16);
-        } else {
+        for (int w = 0; w < WIDE; ++w) one[w] = j + w < dim ? p[j + w] : (typename V::bits)0;
+        return one;
+    };
 #pragma unroll
-            for (int w = 0; w < WIDE; ++w) one[w] = j + w < dim ? p[j + w] : (typename V::bits)0;
-        }
+    for (int i = 0; i < PER; ++i) v[i] = load((i * LANES + lane) * WIDE);
 #pragma unroll
-        for (int w = 0; w < WIDE; ++w) {
-            v[i][w] = V::widen(one[w]);
-            top = max(top, __float_as_uint(v[i][w]) & 0x7fffffffu);
-        }
-    }
+    for (int i = 0; i < PER; ++i) tops = __builtin_elementwise_max(tops, v[i] & (typename V::bits)(V::size == 2 ? 0x7fff : 0x7fffffff));
+    typename V::bits most = tops[0];
+#pragma unroll
+    for (int w = 1; w < WIDE; ++w) most = max(most, tops[w]);
+    uint32_t top = __float_as_uint(V::widen(most));
 #pragma unroll
     for (int o = LANES < 64 ? LANES / 2 : 32; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-    if (LANES == 256) {
+    if (LANES > 64) {
         __shared__ uint32_t s_top[4];
         if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
         __syncthreads();
-        top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+        constexpr uint32_t WAVES = LANES / 64;
+        const uint32_t first = threadIdx.x / LANES * WAVES;
+#pragma unroll
+        for (uint32_t w = 0; w < WAVES; ++w) top = max(top, s_top[first + w]);
     }
     const float big = __uint_as_float(top), s = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : big * PER_STEP;
     if (lane == 0) scales[row] = s;
     const bool some = s > 0.0f;
-    const float up = big < TINY_ROW ? TINY_UP : 1.0f, su = some ? s * up : 1.0f, inv = 1.0f / su, by = some ? up : 0.0f;
+    const float up = big < TINY_ROW ? TINY_UP : 1.0f, su = some ? s * up : 1.0f, inv = 1.0f / su, fast = some ? inv : 0.0f;
+    const float odd = (some && big < TINY_ROW) || s != s ? 1.0f : 0.0f;  // tiny and NaN rows
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const uint32_t j = (i * LANES + lane) * WIDE;
         codes_t q;
+        uint32_t t[WIDE];
+        float worst = odd;
 #pragma unroll
-        for (int w = 0; w < WIDE; ++w) q[w] = (int8_t)(some ? code_of(v[i][w] * by, su, inv) : 0);
+        for (int w = 0; w < WIDE; ++w) {
+            const float y = V::widen(v[i][w]), whole = __builtin_fmaf(y, fast, WHOLE);
+            worst = fmaxf(worst, fabsf(__builtin_fmaf(y, fast, -(whole - WHOLE))));
+            t[w] = __float_as_uint(whole);
+        }
+        if (__any(worst > HALF)) {
+#pragma unroll
+            for (int w = 0; w < WIDE; ++w) t[w] = (uint32_t)(some ? code_of(V::widen(v[i][w]) * up, su, inv) : 0);
+        }
+#pragma unroll
+        for (int w = 0; w < WIDE; w += 4)  // the low bytes
+            q[w / 4] = __builtin_amdgcn_perm(t[w + 1], t[w], 0x0c0c0400u) | __builtin_amdgcn_perm(t[w + 3], t[w + 2], 0x04000c0cu);
+        const uint32_t j = (i * LANES + lane) * WIDE;
         if (j + WIDE <= dim) {
             *(codes_t*)(c + j) = q;
         } else {
 #pragma unroll
             for (int w = 0; w < WIDE; ++w)
-                if (j + w < dim) c[j + w] = q[w];
+                if (j + w < dim) c[j + w] = (int8_t)t[w];
         }
     }
 }
@@ -191,9 +213,13 @@ static hipError_t launch_quantize_rows_of(const typename V::bits* x, uint64_t n,
     else if (loads <= 64) launch_quantize_of<V, 32, 2>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else if (loads <= 96) launch_quantize_of<V, 32, 3>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else if (loads <= 128) launch_quantize_of<V, 64, 2>(x, n, dim, x_stride, codes, c_stride, scales, stream);
+    else if (loads <= 192) launch_quantize_of<V, 64, 3>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else if (loads <= 256) launch_quantize_of<V, 64, 4>(x, n, dim, x_stride, codes, c_stride, scales, stream);
+    else if (loads <= 384) launch_quantize_of<V, 128, 3>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else if (loads <= 512) launch_quantize_of<V, 256, 2>(x, n, dim, x_stride, codes, c_stride, scales, stream);
+    else if (loads <= 768) launch_quantize_of<V, 256, 3>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else if (loads <= 1024) launch_quantize_of<V, 256, 4>(x, n, dim, x_stride, codes, c_stride, scales, stream);
+    else if (loads <= 1536) launch_quantize_of<V, 256, 6>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else if (loads <= 2048) launch_quantize_of<V, 256, 8>(x, n, dim, x_stride, codes, c_stride, scales, stream);
     else hipLaunchKernelGGL((quantize_long_rows_kernel<V>), dim3((uint32_t)std::min<uint64_t>(n, 1u << 16)), dim3(1024), 0, stream, x, n, dim, x_stride, codes, c_stride, scales);
     return hipGetLastError();

@@ -95,6 +95,20 @@ def test_quantize_rows_ties_and_range(ctx, torch):
     assert np.array_equal(codes.cpu().numpy(), want) and not want[-3:].any()
 
 
+@pytest.mark.parametrize("dtype", ("float16", "bfloat16"))
+def test_quantize_rows_of_few_bits(ctx, torch, dtype):
+    """Half-precision values against every significand of the row's largest: quotients that are halves, or nearly so, are
+    common."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = (torch.randn(1024, 640, generator=g, device="cuda") * 0.3).clamp(-1, 1).to(getattr(torch, dtype))
+    x[:, 7] = (1.0 + torch.arange(1024, device="cuda") / 1024).to(getattr(torch, dtype))
+    for rows in (x, x[:, :96].contiguous(), x[::3, 1:]):
+        codes, scales = _quantize(torch, ctx, rows)
+        want, s = _codes_ref(rows.float().cpu().numpy())
+        assert np.array_equal(scales.cpu().numpy(), s)
+        assert np.array_equal(codes.cpu().numpy(), want)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim,x_stride,c_stride,offset", [(33, 50, 41, 1), (384, 400, 384, 0), (256, 257, 259, 3), (64, 64, 128, 0), (1100, 1111, 1101, 5)])
 def test_quantize_rows_that_lie_apart(ctx, torch, dtype, dim, x_stride, c_stride, offset):
