@@ -639,9 +639,8 @@ static hipError_t launch_stream_of(const MatmulParams& p, hipStream_t stream) {
 static bool rows_aligned(const MatmulParams& p) {
     return p.k % 16 == 0 && p.a_stride % 16 == 0 && p.b_stride % 16 == 0 && (uintptr_t)p.a % 16 == 0 && (uintptr_t)p.b % 16 == 0;
 }
-static bool fills_big_tiles(const MatmulParams& p, int n_cu) {
-    return p.m > 128 && p.k >= 512 && ((p.n + 255) / 256) * ((p.m + 255) / 256) >= (uint64_t)n_cu;
-}
+static uint64_t tiles_of(const MatmulParams& p, uint64_t tb, uint64_t ta) { return ((p.n + tb - 1) / tb) * ((p.m + ta - 1) / ta); }
+
 template <typename V>
 static hipError_t launch_matmul_of(const MatmulParams& p, int n_cu, hipStream_t stream) {
     const bool aligned = rows_aligned(p);
@@ -652,14 +651,19 @@ static hipError_t launch_matmul_of(const MatmulParams& p, int n_cu, hipStream_t 
         return p.n < 64ull * n_cu ? launch_stream_of<V, 2, 1, true>(p, stream) : launch_stream_of<V, 4, 1, true>(p, stream);
     }
     // Tiles, by what fills the chip (us of the kernel, sizes m x n x k).  A long product of many 256 x 256 tiles is bound by the
-    // matrix cores and the power they draw: 8192 x 8192 x 4096 takes 247 with them, 480 with 128 x 128.  Shorter or fewer:
-    // 128 x 128 (2048 x 2048 x 2048: 21, against 24 with 128 x 64 and 38 with 256 x 256; 1000 x 100000 x 128, bound by its
-    // output: 98, against 110 with 256 x 256); below half a tile per CU 128 x 64 and 64 x 64 (512 x 512 x 4096: 18 with
-    // 64 x 64, 25 with 128 x 128).
-    const auto tiles = [&](uint64_t tb, uint64_t ta) { return ((p.n + tb - 1) / tb) * ((p.m + ta - 1) / ta); };
+    // matrix cores and the power they draw: 8192 x 8192 x 4096 takes 247 with them, 480 with 128 x 128.  One such tile per CU
+    // takes about (2.8 + 512 / k) times one of 128 x 128 per CU, and what counts is how often the chip is filled: 4096 x
+    // 4096 x 2048 (1 and 4 fills) 32 with 256 x 256, 38 with 128 x 128; 4096 x 4352 x 2048 (2 and 5) 57 and 46; 4096 x 6144 x
+    // 4096 (2 and 6) 106 and 115; 2048 x 2048 x 2048 38 and 21.  Short ones: 1000 x 100000 x 128, bound by its output, 110 and
+    // 98.  Below half a tile per CU 128 x 64 and 64 x 64 (512 x 512 x 4096: 18 with 64 x 64, 25 with 128 x 128).  Through
+    // registers 256 x 128 are the largest, and taken where they come to two per CU.
+    const auto tiles = [&](uint64_t tb, uint64_t ta) { return tiles_of(p, tb, ta); };
     const uint64_t cu = (uint64_t)n_cu;
-    if (fills_big_tiles(p, n_cu))
-        return aligned ? launch_tiles_of<V, 256, 256, 2, 4, 4, true>(p, stream) : launch_tiles_of<V, 256, 128, 4, 2, 4, false>(p, stream);
+    const auto fills = [&](uint64_t of) { return (of + cu - 1) / cu; };
+    if (p.m > 128 && p.k >= 512) {
+        if (aligned && (28 + 5120 / p.k) * fills(tiles(256, 256)) < 10 * fills(tiles(128, 128))) return launch_tiles_of<V, 256, 256, 2, 4, 4, true>(p, stream);
+        if (!aligned && tiles(256, 256) >= cu) return launch_tiles_of<V, 256, 128, 4, 2, 4, false>(p, stream);
+    }
     if (p.m > 64 && tiles(128, 128) >= cu / 2)
         return aligned ? launch_tiles_of<V, 128, 128, 4, 2, 4, true>(p, stream) : launch_tiles_of<V, 128, 128, 4, 2, 4, false>(p, stream);
     if (tiles(128, 64) >= cu)
@@ -676,8 +680,8 @@ static hipError_t launch_slab(needle_hip_ctx* c, MatmulParams p, int out_value) 
     // product through registers: 8192 x 8192 x 1000 104, 145; 2256 x 6573 x 1946 62, 83; 4196 x 5755 x 218 28, 34; 600 x 60000 x
     // 513 62, 64; not so 300 x 66000 x 513 63, 46; 2000 x 2000 x 301 11, 7.
     const uint32_t stride = (p.k + 63) / 64 * 64;
-    const uint64_t bytes = (p.n + p.m) * stride, tiles = ((p.n + 127) / 128) * ((p.m + 127) / 128);
-    if (!rows_aligned(p) && tiles > (uint64_t)c->n_cu && p.m * p.n >= 512 * (p.m + p.n) && bytes <= ALIGN_MOST) {
+    const uint64_t bytes = (p.n + p.m) * stride;
+    if (!rows_aligned(p) && tiles_of(p, 128, 128) > (uint64_t)c->n_cu && p.m * p.n >= 512 * (p.m + p.n) && bytes <= ALIGN_MOST) {
         const hipError_t e = c->scratch[5].ensure(bytes);
         if (e != hipSuccess) return e;
         int8_t* to = c->scratch[5].as<int8_t>();
