@@ -37,11 +37,13 @@ typedef u32x4 u32x4_any __attribute__((aligned(1)));
 // The same 16 bytes where the address need not even be a multiple of four.  A load from such an address is taken apart by the
 // memory pipeline (1 x 9856 x 3569 codes of odd stride: 32 us with it, 19 with this): so the whole words that hold the bytes are
 // read and shifted into place.  No word without one of the bytes is read.
+typedef __attribute__((address_space(1))) uint32_t global_words;
+typedef u32x4 u32x4_words __attribute__((aligned(4)));
+typedef __attribute__((address_space(1))) u32x4_words global_words4;
 __device__ inline u32x4 load16_odd(const void* p) {
-    typedef u32x4 u32x4_words __attribute__((aligned(4)));
     const uint32_t by = (uint32_t)(uint64_t)p & 3;
-    const uint32_t* q = (const uint32_t*)((uint64_t)p & ~3ull);
-    const u32x4 v = *(const u32x4_words*)q;
+    const global_words* q = (const global_words*)((uint64_t)p & ~3ull);
+    const u32x4 v = *(const global_words4*)q;
     const uint32_t w = q[by ? 4 : 3];
     return u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], by), __builtin_amdgcn_alignbyte(v[2], v[1], by),
                  __builtin_amdgcn_alignbyte(v[3], v[2], by), __builtin_amdgcn_alignbyte(w, v[3], by)};

@@ -188,7 +188,9 @@ def test_matmul(ctx, torch, m, n, k):
 
 @pytest.mark.parametrize("m,n,k,a_stride,b_stride,o_stride,offset", [
     (5, 70, 64, 96, 80, 70, 0), (37, 501, 301, 384, 384, 501, 0), (3, 129, 48, 49, 51, 131, 1), (70, 200, 256, 272, 257, 203, 16),
-    (300, 300, 128, 144, 128, 304, 0), (260, 300, 144, 160, 176, 302, 16), (1, 65, 200, 200, 203, 65, 7), (130, 140, 33, 64, 64, 140, 0)])
+    (300, 300, 128, 144, 128, 304, 0), (260, 300, 144, 160, 176, 302, 16), (1, 65, 200, 200, 203, 65, 7), (130, 140, 33, 64, 64, 140, 0),
+    (40, 50, 7, 16, 16, 50, 0), (17, 33, 1, 16, 32, 33, 0), (100, 90, 515, 528, 528, 90, 0), (60, 20_000, 255, 256, 272, 20_000, 0),
+    (520, 6000, 1009, 1024, 1024, 6000, 16), (2040, 8190, 529, 544, 560, 8190, 0), (2040, 8190, 528, 544, 560, 8190, 0)])
 def test_matmul_rows_that_lie_apart(ctx, torch, m, n, k, a_stride, b_stride, o_stride, offset):
     g = torch.Generator(device="cuda").manual_seed(m + n + k)
     a, sa = _table(torch, g, m, k, a_stride, offset)
