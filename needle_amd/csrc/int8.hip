@@ -389,19 +389,21 @@ __global__ __launch_bounds__(256) void matmul_i8_stream_kernel(MatmulParams p) {
 // chunk c of row r at place c ^ 2 (r >> 3 & 1): the sixteen 16-byte reads that meet the banks together touch all of them
 // once.  DMA: the loads write LDS themselves (rows aligned to 16 bytes, the end of a row of other than a multiple of 16 apart;
 // 300 x 20000 x 777 of stride 784: 15 us, 18 through registers); otherwise they pass through registers two slices ahead,
-// from any address.
+// from any address.  SHARES: so many times the waves, each share with slots of its own and every SHARES-th slice; their sums
+// meet in LDS at the end (whole numbers: any order is exact).
 constexpr uint32_t SLICE = 64;
 __device__ const uint32_t g_zeros[4] = {0, 0, 0, 0};
 typedef __attribute__((address_space(1))) const void glb_cvoid;
 typedef __attribute__((address_space(3))) void lds_void;
 
-template <typename V, int TB, int TA, int WB, int WA, int SLOTS, bool DMA>
-__global__ __launch_bounds__(64 * WB * WA) void matmul_i8_tile_kernel(MatmulParams p, uint32_t tiles_b, uint32_t tiles_a) {
+template <typename V, int TB, int TA, int WB, int WA, int SLOTS, bool DMA, int SHARES>
+__global__ __launch_bounds__(64 * WB * WA * SHARES) void matmul_i8_tile_kernel(MatmulParams p, uint32_t tiles_b, uint32_t tiles_a) {
     constexpr int WAVES = WB * WA, NB = TB / WB / 16, NA = TA / WA / 16, STAGE = (TB + TA) * SLICE, LOADS = (TB + TA) / 16 / WAVES;
     static_assert((TB + TA) % (16 * WAVES) == 0 && TB % 16 == 0, "every wave fills whole groups of sixteen rows");
-    extern __shared__ __align__(16) uint8_t s_tile[];
-    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, l15 = lane & 15, quad = lane >> 4;
+    extern __shared__ __align__(16) uint8_t s_tiles[];
+    const uint32_t t = threadIdx.x, lane = t & 63, wave = (t >> 6) % WAVES, share = (t >> 6) / WAVES, l15 = lane & 15, quad = lane >> 4;
     const uint32_t wb = wave % WB, wa = wave / WB;
+    uint8_t* s_tile = s_tiles + share * (SLOTS * STAGE);
     // Workgroups go to the chip's eight dies in turn, each with its own L2: a die gets a run of tiles, in groups of four
     // tiles of a that share their tiles of b.
     const uint32_t tiles = tiles_b * tiles_a;
@@ -422,11 +424,13 @@ __global__ __launch_bounds__(64 * WB * WA) void matmul_i8_tile_kernel(MatmulPara
         const uint32_t r = (wave + i * WAVES) * 16 + (lane >> 2);
         from[i] = r < TB ? p.b + min(n0 + r, p.n - 1) * p.b_stride : p.a + (uint64_t)min(m0 + r - TB, p.m - 1) * p.a_stride;
     }
-    const uint32_t slices = (p.k + SLICE - 1) / SLICE, whole = p.k % 16 ? p.k / SLICE : slices;
+    // this share's slices; how many of them the loads write themselves
+    const uint32_t slices = ((p.k + SLICE - 1) / SLICE + SHARES - 1) / SHARES, full = p.k / SLICE;
+    const uint32_t whole = p.k % 16 == 0 ? slices : full > share ? (full - share + SHARES - 1) / SHARES : 0;
     auto fill = [&](uint32_t s) {
         uint8_t* to = s_tile + s % SLOTS * STAGE + wave * 1024;
-        const uint32_t at = s * SLICE + chunk;
-        if ((s + 1) * SLICE <= p.k) {
+        const uint32_t at0 = (s * SHARES + share) * SLICE, at = at0 + chunk;
+        if (at0 + SLICE <= p.k) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i)
                 __builtin_amdgcn_global_load_lds((glb_cvoid*)(from[i] + at), (lds_void*)(to + i * WAVES * 1024), 16, 0, 0);
@@ -447,7 +451,7 @@ __global__ __launch_bounds__(64 * WB * WA) void matmul_i8_tile_kernel(MatmulPara
         for (int i = 0; i < LOADS; ++i) *(u32x4*)(to + lane * 16 + i * WAVES * 1024) = end[i];
     };
     auto fetch = [&](uint32_t s, u32x4 (&held)[LOADS]) {
-        const uint32_t at = s * SLICE;
+        const uint32_t at = (s * SHARES + share) * SLICE;
         if (at + SLICE <= p.k) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) held[i] = *(const u32x4_any*)(from[i] + at + chunk);
@@ -542,6 +546,26 @@ __global__ __launch_bounds__(64 * WB * WA) void matmul_i8_tile_kernel(MatmulPara
         }
         if (s < slices) step(s, 0);
     }
+    if (SHARES > 1) {  // the sums of the other shares meet in LDS
+        i32x4* sums = (i32x4*)s_tiles + (wave * 64 + lane);
+        constexpr uint32_t STEP = WAVES * 64;
+        __syncthreads();
+        if (share) {
+#pragma unroll
+            for (int x = 0; x < NB; ++x)
+#pragma unroll
+                for (int y = 0; y < NA; ++y) sums[((share - 1) * NB * NA + x * NA + y) * STEP] = acc[x][y];
+        }
+        __syncthreads();
+        if (!share) {
+#pragma unroll
+            for (int o = 0; o < SHARES - 1; ++o)
+#pragma unroll
+                for (int x = 0; x < NB; ++x)
+#pragma unroll
+                    for (int y = 0; y < NA; ++y) acc[x][y] += sums[(o * NB * NA + x * NA + y) * STEP];
+        }
+    }
     const uint64_t j0 = n0 + wb * (TB / WB) + quad * 4;
     const uint32_t i0 = m0 + wa * (TA / WA) + l15;
     f32x4_any sb[NB], bias[NB];
@@ -569,6 +593,7 @@ __global__ __launch_bounds__(64 * WB * WA) void matmul_i8_tile_kernel(MatmulPara
         static_assert(ROWS * LINE * WAVES <= SLOTS * STAGE && CHUNKS <= 64 && ROWS % GO == 0, "the waves' parts fit");
         uint8_t* part = s_tile + wave * (ROWS * LINE);
         __syncthreads();
+        if (share) return;
         o = (typename V::bits*)p.out + (uint64_t)(m0 + wa * (TA / WA)) * p.out_stride + n0 + wb * (TB / WB);
 #pragma unroll
         for (int y0 = 0; y0 < NA; y0 += PASS) {
@@ -595,7 +620,7 @@ __global__ __launch_bounds__(64 * WB * WA) void matmul_i8_tile_kernel(MatmulPara
             }
             __builtin_amdgcn_wave_barrier();
         }
-    } else {
+    } else if (!share) {
 #pragma unroll
         for (int y = 0; y < NA; ++y) {
             if (i0 + y * 16 >= p.m) continue;
@@ -615,18 +640,21 @@ __global__ __launch_bounds__(64 * WB * WA) void matmul_i8_tile_kernel(MatmulPara
     }
 }
 
-template <typename V, int TB, int TA, int WB, int WA, int SLOTS, bool DMA>
+template <typename V, int TB, int TA, int WB, int WA, int SLOTS, bool DMA, int SHARES = 1>
 static hipError_t launch_tiles_of(const MatmulParams& p, hipStream_t stream) {
-    constexpr uint32_t lds = SLOTS * (TB + TA) * SLICE;
+    constexpr uint32_t lds = SHARES * SLOTS * (TB + TA) * SLICE;
     if (lds >= 65536) {  // (per device, like every attribute of a kernel)
         const hipError_t e =
-            hipFuncSetAttribute((const void*)matmul_i8_tile_kernel<V, TB, TA, WB, WA, SLOTS, DMA>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            hipFuncSetAttribute((const void*)matmul_i8_tile_kernel<V, TB, TA, WB, WA, SLOTS, DMA, SHARES>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
     const uint32_t tiles_b = (uint32_t)((p.n + TB - 1) / TB), tiles_a = (p.m + TA - 1) / TA;
-    hipLaunchKernelGGL((matmul_i8_tile_kernel<V, TB, TA, WB, WA, SLOTS, DMA>), dim3(tiles_b * tiles_a), dim3(64 * WB * WA), lds, stream, p, tiles_b, tiles_a);
+    hipLaunchKernelGGL((matmul_i8_tile_kernel<V, TB, TA, WB, WA, SLOTS, DMA, SHARES>), dim3(tiles_b * tiles_a), dim3(64 * WB * WA * SHARES), lds, stream, p, tiles_b, tiles_a);
     return hipGetLastError();
 }
+// From this k on the few tiles of a small product share it among four times the waves: 512 x 512 x 4096 takes 13 us so, 18
+// without; 64 x 1000 x 4096 9 and 14; 500 x 700 x 768 5 either way, 1000 x 1000 x 1024 7.5 and 6.6.
+constexpr uint32_t SHARED_K = 2048;
 constexpr uint64_t ALIGN_MOST = 2ull << 30;  // workspace of the aligned copies; beyond it the rows pass through registers
 // The rows of b and of a copied to rows of `to_stride` (a multiple of 64) with zeros behind them, a wave per row.
 __global__ __launch_bounds__(256) void align_rows_kernel(MatmulParams p, int8_t* __restrict__ to, uint32_t to_stride) {
@@ -668,7 +696,7 @@ static hipError_t launch_matmul_of(const MatmulParams& p, int n_cu, hipStream_t 
     // takes about (2.8 + 512 / k) times one of 128 x 128 per CU, and what counts is how often the chip is filled: 4096 x
     // 4096 x 2048 (1 and 4 fills) 32 with 256 x 256, 38 with 128 x 128; 4096 x 4352 x 2048 (2 and 5) 57 and 46; 4096 x 6144 x
     // 4096 (2 and 6) 106 and 115; 2048 x 2048 x 2048 38 and 21.  Short ones: 1000 x 100000 x 128, bound by its output, 110 and
-    // 98.  Below half a tile per CU 128 x 64 and 64 x 64 (512 x 512 x 4096: 18 with 64 x 64, 25 with 128 x 128).  Through
+    // 98.  Below half a tile per CU 128 x 64 and 64 x 64 (512 x 512 x 4096: 18 with 64 x 64 and one share, 25 with 128 x 128).  Through
     // registers 256 x 128 are the largest, and taken where they come to two per CU.
     const auto tiles = [&](uint64_t tb, uint64_t ta) { return tiles_of(p, tb, ta); };
     const uint64_t cu = (uint64_t)n_cu;
@@ -681,6 +709,8 @@ static hipError_t launch_matmul_of(const MatmulParams& p, int n_cu, hipStream_t 
         return aligned ? launch_tiles_of<V, 128, 128, 4, 2, 4, true>(p, stream) : launch_tiles_of<V, 128, 128, 4, 2, 4, false>(p, stream);
     if (tiles(128, 64) >= cu)
         return aligned ? launch_tiles_of<V, 128, 64, 2, 2, 4, true>(p, stream) : launch_tiles_of<V, 128, 64, 2, 2, 4, false>(p, stream);
+    if (p.k >= SHARED_K && tiles(64, 64) <= cu)
+        return aligned ? launch_tiles_of<V, 64, 64, 2, 2, 4, true, 4>(p, stream) : launch_tiles_of<V, 64, 64, 2, 2, 4, false, 4>(p, stream);
     return aligned ? launch_tiles_of<V, 64, 64, 2, 2, 4, true>(p, stream) : launch_tiles_of<V, 64, 64, 2, 2, 4, false>(p, stream);
 }
 static hipError_t launch_slab(needle_hip_ctx* c, MatmulParams p, int out_value) {

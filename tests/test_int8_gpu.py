@@ -171,7 +171,8 @@ def _check_product(out, a, sa, b, sb, bias, dtype):
 SHAPES = [(1, 1, 1), (1, 17, 16), (3, 5, 7), (16, 16, 64), (17, 33, 65), (1, 1000, 128), (4, 130, 1024), (5, 2049, 384), (64, 64, 63), (65, 127, 300),
           (128, 128, 128), (130, 257, 256), (200, 700, 80), (256, 256, 512), (257, 513, 1008), (300, 1000, 1000), (1, 300, 4096), (16, 515, 5000),
           (33, 64, 2048), (512, 768, 272), (70, 40, 16), (1000, 3, 96), (2, 9, 9999), (4112, 4097, 528), (4100, 4105, 513), (1500, 1700, 192), (1500, 1701, 67), (50, 33_000, 96),
-          (20, 20_000, 33), (16, 17_000, 400), (7, 20_000, 700)]
+          (20, 20_000, 33), (16, 17_000, 400), (7, 20_000, 700), (40, 50, 4097), (65, 130, 2064), (100, 90, 9000), (64, 128, 2112), (130, 1000, 2048),
+          (20, 30, 131_071)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -190,7 +191,8 @@ def test_matmul(ctx, torch, m, n, k):
     (5, 70, 64, 96, 80, 70, 0), (37, 501, 301, 384, 384, 501, 0), (3, 129, 48, 49, 51, 131, 1), (70, 200, 256, 272, 257, 203, 16),
     (300, 300, 128, 144, 128, 304, 0), (260, 300, 144, 160, 176, 302, 16), (1, 65, 200, 200, 203, 65, 7), (130, 140, 33, 64, 64, 140, 0),
     (40, 50, 7, 16, 16, 50, 0), (17, 33, 1, 16, 32, 33, 0), (100, 90, 515, 528, 528, 90, 0), (60, 20_000, 255, 256, 272, 20_000, 0),
-    (520, 6000, 1009, 1024, 1024, 6000, 16), (2040, 8190, 529, 544, 560, 8190, 0), (2040, 8190, 528, 544, 560, 8190, 0)])
+    (520, 6000, 1009, 1024, 1024, 6000, 16), (2040, 8190, 529, 544, 560, 8190, 0), (2040, 8190, 528, 544, 560, 8190, 0), (100, 90, 2500, 2512, 2528, 90, 0),
+    (64, 64, 2049, 2064, 2064, 64, 0), (200, 300, 3333, 3344, 3333, 300, 0), (64, 64, 2240, 2240, 2256, 64, 16)])
 def test_matmul_rows_that_lie_apart(ctx, torch, m, n, k, a_stride, b_stride, o_stride, offset):
     g = torch.Generator(device="cuda").manual_seed(m + n + k)
     a, sa = _table(torch, g, m, k, a_stride, offset)
