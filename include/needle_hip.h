@@ -563,7 +563,11 @@ needle_hip_status needle_hip_linear_i8_device(needle_hip_ctx* ctx, const void* d
  *     normalize 0: scores[row] + x        normalize 1: scores[row] + (x - log sum exp x)
  * with the sum over the row's admitted continuations.  The k best of a group by (total
  * descending, beam, token) are its picks; continuations of one beam rank by their logits.
- * Totals are formed and compared in 64 bits and reported rounded to f32.  Not offered: what the mask leaves out, totals of -inf or
+ * Totals are formed and compared in 64-bit floating point, exponentials and sums among them, and
+ * reported rounded to f32.  A row of which one continuation counts gives it a log-probability of
+ * exactly 0, so that its total equals an ended beam's of the same score; apart from such sums, and
+ * from rows of equal sums, totals of different beams that lie closer than about 1e-14 may come in
+ * either order (the same on every run).  Not offered: what the mask leaves out, totals of -inf or
  * NaN (so a beam whose score is -inf or NaN offers nothing; nor does, under normalize, a
  * row with an admitted NaN or +inf).  An ended beam offers one continuation: end_token
  * with scores[row] as its total; its row of logits and its mask are not looked at.

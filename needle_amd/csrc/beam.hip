@@ -8,10 +8,9 @@
 // pieces of a group.  The pass is bound by the bytes of the logits.
 //
 // Picks are whole numbers and two beams' totals may lie a rounding apart, so all that decides between beams is held in 64
-// bits: the exponentials, their sums, the totals.  An f64 instruction takes twice the cycles of an f32 one here, and about
-// fourteen of them per logit bound the kernel where it takes a log-softmax of half-precision logits (67 us for 64 x 8 rows
-// of 131072 bf16 logits; an f32 polynomial for all but the largest terms took 60 us, and erred by 1e-7 in the log where
-// thousands of logits are equal).
+// bits: the exponentials (a few units in the last place each), their sums, the totals.  A sum is held in units of its largest
+// term, which so adds exactly 1: a row of which one continuation counts has the logarithm of 1, and its total is its score, as
+// an ended beam's is.
 #include "nh_values.h"
 
 namespace nh {
@@ -19,24 +18,52 @@ namespace nh {
 constexpr uint32_t BEAM_K_MAX = 256, BEAMS_MAX = 1024;
 constexpr uint32_t PIECE_THREADS = 256;
 
-// ---- exponential of x <= 64 in 64 bits -------------------------------------------------------
+// ---- exponential of x <= 0 in 64 bits --------------------------------------------------------
 // exp x = 2^n 2^f with n the whole number nearest to x / ln 2 (found by adding 1.5 * 2^52, which leaves it in the low
-// bits of the sum) and 2^f, |f| <= 1/2, by a polynomial of degree 7 that equals it at the eight Chebyshev nodes: at most
-// 5.6e-11 of the result off, with changing sign.  Below -700 the result is that of -700, 1e-304: nothing beside a 1.
+// bits of the sum), |f| <= 1/2, and 2^f = 1 + f g(f) with g interpolated at eleven Chebyshev nodes: 2e-17 of the result
+// off besides the roundings, and exactly 1 at 0.  Below -700 the result is that of -700, 1e-304: nothing beside a 1.
+constexpr double ONE_AND_A_HALF = 6755399441055744.0, PER_LN2 = 1.4426950408889634074;
+__device__ inline double add_to_high(double d, int n) { return __hiloint2double(__double2hiint(d) + n, __double2loint(d)); }
+__device__ inline double exp2_near_0(double f) {
+    double g = 0x1.e9d3fe3952179p-32;
+    g = __builtin_fma(g, f, 0x1.e6063f7217bc6p-28);
+    g = __builtin_fma(g, f, 0x1.b524fae627834p-24);
+    g = __builtin_fma(g, f, 0x1.62bfd47773353p-20);
+    g = __builtin_fma(g, f, 0x1.ffcbfc670dcd4p-17);
+    g = __builtin_fma(g, f, 0x1.430913096fd9fp-13);
+    g = __builtin_fma(g, f, 0x1.5d87fe78a5276p-10);
+    g = __builtin_fma(g, f, 0x1.3b2ab6fba1ddap-7);
+    g = __builtin_fma(g, f, 0x1.c6b08d704a0c2p-5);
+    g = __builtin_fma(g, f, 0x1.ebfbdff82c598p-3);
+    g = __builtin_fma(g, f, 0x1.62e42fefa39efp-1);
+    return __builtin_fma(g, f, 1.0);
+}
 __device__ inline double exp64(double x) {
-    constexpr double ONE_AND_A_HALF = 6755399441055744.0, PER_LN2 = 1.4426950408889634074;
     x = fmax(x, -700.0);
     const double s = __builtin_fma(x, PER_LN2, ONE_AND_A_HALF);
-    const double f = __builtin_fma(x, PER_LN2, -(s - ONE_AND_A_HALF));
-    double p = 0x1.00c0e4e15189cp-16;
-    p = __builtin_fma(p, f, 0x1.446c79efd4834p-13);
-    p = __builtin_fma(p, f, 0x1.5d877598350dep-10);
-    p = __builtin_fma(p, f, 0x1.3b29d8bb0b97ep-7);
-    p = __builtin_fma(p, f, 0x1.c6b08da70cce3p-5);
-    p = __builtin_fma(p, f, 0x1.ebfbe0aa03df0p-3);
-    p = __builtin_fma(p, f, 0x1.62e42fef9cc69p-1);
-    p = __builtin_fma(p, f, 0x1.ffffffffa7135p-1);
-    return __hiloint2double(__double2hiint(p) + (__double2loint(s) << 20), __double2loint(p));
+    return add_to_high(exp2_near_0(__builtin_fma(x, PER_LN2, -(s - ONE_AND_A_HALF))), (int)((uint32_t)__double2loint(s) << 20));
+}
+// The same with the 128 powers 2^(j / 128) in LDS, for one exponential per logit: n counts 128ths, and what is left is so
+// small that g takes four nodes (1.5e-16); with the roundings e^x is 4 + |x| units of 2^-53 off at most.  A power lies there
+// less its number j in the exponent's lowest bits, so that adding n there gives 2^(n / 128).  Twelve f64 instructions per
+// logit, its place in the sum among them; without powers it would be eighteen (64 x 8 rows of 131072 bf16 logits: 8 us more).
+constexpr int POWER_BITS = 7, POWERS = 1 << POWER_BITS;
+__device__ inline void fill_powers(double* powers, int t) {
+    if (t >= POWERS) return;
+    const double power = t <= POWERS / 2 ? exp2_near_0(t * (1.0 / POWERS)) : 2.0 * exp2_near_0(t * (1.0 / POWERS) - 1.0);
+    powers[t] = add_to_high(power, -(t << (20 - POWER_BITS)));
+}
+__device__ inline double exp64(double x, const double* powers) {
+    x = fmax(x, -700.0);
+    const double s = __builtin_fma(x, POWERS * PER_LN2, ONE_AND_A_HALF);
+    const double f = __builtin_fma(x, POWERS * PER_LN2, -(s - ONE_AND_A_HALF));
+    const int n = __double2loint(s);
+    double g = 0x1.3b2abc07c93d0p-35;
+    g = __builtin_fma(g, f, 0x1.c6b0985c8a1bcp-26);
+    g = __builtin_fma(g, f, 0x1.ebfbdff82c4edp-17);
+    g = __builtin_fma(g, f, 0x1.62e42fefa3892p-8);
+    const double power = add_to_high(powers[n & (POWERS - 1)], (int)((uint32_t)n << (20 - POWER_BITS)));
+    return __builtin_fma(power, g * f, power);
 }
 
 // order-preserving whole number of a double (-0 as +0); 0 for what is never offered (-inf, NaN)
@@ -138,7 +165,8 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
     __shared__ __align__(16) uint64_t s_list[CAP + 8];
     __shared__ double s_sum[4];
     __shared__ float s_top[4];
-    __shared__ uint32_t s_nan, s_add[3], s_bound, s_fill;
+    __shared__ double s_powers[NORMALIZE ? POWERS : 1];
+    __shared__ uint32_t s_nan, s_add[3], s_bound, s_highest, s_fill;
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const uint32_t row = blockIdx.x / p.pieces, piece = blockIdx.x % p.pieces;
     const size_t at = (size_t)row * p.pieces + piece;
@@ -175,19 +203,22 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
         }
     };
     load(first);
+    if (NORMALIZE) fill_powers(s_powers, (int)t);  // (the first bound's barriers stand before their use)
 
     uint32_t n = 0;      // entries of the list
     float bound = 0.0f;  // a logit below it is not among the k largest
     float run[GROUPS];   // largest logits of this thread so far
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) run[g] = -__builtin_inff();
-    // the thread's sum of exponentials, in units of exp(ref)
+    // The thread's sum of exponentials, in units of exp(ref): ref is the largest logit of the workgroup when the bound was last
+    // raised, or a larger one of this thread since.  (In units of the thread's own largest, which grows in most of the first
+    // chunks, 64 x 8 rows of 131072 logits take 2.5 us longer in f32, 0.5 in bf16.)
     double sum = 0.0;
-    float ref = -__builtin_inff();
+    float ref = -__builtin_inff(), highest = ref;
     bool nan = false;
     uint32_t slot = 0;
 
-    // bound := the k-th largest running maximum
+    // bound := the k-th largest running maximum; s_highest: the largest
     auto raise = [&] {
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) s_max[g * PIECE_THREADS + t] = run[g] > -__builtin_inff() ? f2ord(run[g] + 0.0f) : 0;
@@ -195,6 +226,12 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
         if (wave == 0) {
             const uint32_t kth = kth_largest<4 * GROUPS>(s_max, p.k, lane);
             if (lane == 0) s_bound = max(kth, LOWEST);
+        } else if (NORMALIZE && wave == 1) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 4 * GROUPS; ++i) m = max(m, s_max[lane + 64 * i]);
+            m = wave_max(m);
+            if (lane == 0) s_highest = m;
         }
         __syncthreads();
         return ord2f(s_bound);
@@ -260,6 +297,7 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
         if ((done & (done - 1)) == 0) {
             const float b = raise();
             bound = done == 1 ? b : fmaxf(bound, b);
+            if (NORMALIZE && s_highest) highest = ord2f(s_highest);
         }
         // the logits that reach `least` go behind the list's n entries: one place per wave, then one per logit; how many
         auto append = [&](float least) {
@@ -323,14 +361,15 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
         }
         n += add;
         if (NORMALIZE && top > -__builtin_inff()) {
-            if (!(top - ref <= 64.0f)) {  // ref is -inf at first
-                sum = ref > -__builtin_inff() ? sum * exp64((double)ref - (double)top) : 0.0;
-                ref = top;
+            const float most = fmaxf(top, highest);
+            if (most > ref) {  // ref is -inf at first, and the sum 0
+                sum *= exp64((double)ref - (double)most, s_powers);
+                ref = most;
             }
             const double r = (double)ref;
 #pragma unroll
             for (int e = 0; e < EACH; ++e) {
-                sum += exp64((double)v[e] - r);
+                sum += exp64((double)v[e] - r, s_powers);
                 if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: more in flight cost registers, and waves
             }
         }
