@@ -125,16 +125,16 @@ __global__ __launch_bounds__(1024) void quantize_long_rows_kernel(const typename
     for (uint64_t row = blockIdx.x; row < n; row += gridDim.x) {
         const typename V::bits* p = x + row * x_stride;
         int8_t* c = codes + row * c_stride;
-        const uint32_t whole = dim / WIDE * WIDE;
+        const uint32_t whole = dim / WIDE * WIDE, left = dim - whole;
         uint32_t top = 0;
-        for (uint32_t j = t * WIDE; j < whole; j += AT_ONCE) {
+        for (uint64_t j = t * WIDE; j < whole; j += AT_ONCE) {  // (64 bits: a step past a long row's end)
             const u32x4 raw = *(const u32x4_any*)(p + j);
             typename V::bits one[WIDE];
             __builtin_memcpy(one, &raw, 16);
 #pragma unroll
             for (int w = 0; w < (int)WIDE; ++w) top = max(top, __float_as_uint(V::widen(one[w])) & 0x7fffffffu);
         }
-        if (whole + t < dim) top = max(top, __float_as_uint(V::widen(p[whole + t])) & 0x7fffffffu);
+        if (t < left) top = max(top, __float_as_uint(V::widen(p[whole + t])) & 0x7fffffffu);
         for (int o = 32; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
         __syncthreads();  // (the row before has left s_top)
         if ((t & 63) == 0) s_top[t >> 6] = top;
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(1024) void quantize_long_rows_kernel(const typename
         if (t == 0) scales[row] = s;
         const bool some = s > 0.0f;
         const float up = big < TINY_ROW ? TINY_UP : 1.0f, su = some ? s * up : 1.0f, inv = 1.0f / su;
-        for (uint32_t j = t * WIDE; j < whole; j += AT_ONCE) {
+        for (uint64_t j = t * WIDE; j < whole; j += AT_ONCE) {
             const u32x4 raw = *(const u32x4_any*)(p + j);
             typename V::bits one[WIDE];
             __builtin_memcpy(one, &raw, 16);
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(1024) void quantize_long_rows_kernel(const typename
             for (int w = 0; w < (int)WIDE; ++w) q[w] = (int8_t)(some ? code_of(V::widen(one[w]) * up, su, inv) : 0);
             *(codes_t*)(c + j) = q;
         }
-        if (whole + t < dim) c[whole + t] = (int8_t)(some ? code_of(V::widen(p[whole + t]) * up, su, inv) : 0);
+        if (t < left) c[whole + t] = (int8_t)(some ? code_of(V::widen(p[whole + t]) * up, su, inv) : 0);
     }
 }
 
@@ -201,7 +201,7 @@ static void launch_quantize_of(const typename V::bits* x, uint64_t n, uint32_t d
 template <typename V>
 static hipError_t launch_quantize_rows_of(const typename V::bits* x, uint64_t n, uint32_t dim, uint64_t x_stride, int8_t* codes, uint64_t c_stride,
                                           float* scales, hipStream_t stream) {
-    const uint32_t loads = (dim + 16 / V::size - 1) / (16 / V::size);  // of a row
+    const uint32_t loads = (uint32_t)(((uint64_t)dim + 16 / V::size - 1) / (16 / V::size));  // of a row
     // several loads per lane where the row has them, few idle lanes: us of 1000000 x 64 f32 with <4, 2>, <8, 1>: 56, 69 (less a
     // call's 17); 100000 x 384 f16 with <16, 3>, <32, 2>: 24, 34; 3000000 x 24 bf16 with <4, 1>, <8, 1>: 64, 128; 16384 x 4096
     // bf16 with <256, 2>, <64, 8>: 41, 44; 30000 x 1000 f32 with <64, 4>, <256, 1>: 23, 30

@@ -95,6 +95,27 @@ def test_quantize_rows_ties_and_range(ctx, torch):
     assert np.array_equal(codes.cpu().numpy(), want) and not want[-3:].any()
 
 
+@pytest.mark.parametrize("dtype,dim", [("float16", 2 ** 32 - 1), ("bfloat16", 2 ** 32 - 8190), ("float32", 2 ** 31 + 5)])
+def test_quantize_a_row_of_billions(ctx, torch, dtype, dim):
+    """A row that ends within one step of 2^32 values, where a 32-bit place would wrap, and one longer than 2^31."""
+    t = getattr(torch, dtype)
+    g = torch.Generator(device="cuda").manual_seed(dim % 1000)
+    x = torch.empty(1, dim, dtype=t, device="cuda")
+    some = torch.randn(1 << 24, generator=g, device="cuda").clamp_(-5, 5).to(t)
+    for at in range(0, dim, some.numel()):
+        x[0, at:at + some.numel()] = some[:min(some.numel(), dim - at)]
+    x[0, dim - 2] = -7.0
+    codes, scales = _quantize(torch, ctx, x)
+    s = np.float32(7) * (np.float32(1) / np.float32(127))
+    assert float(scales[0]) == float(s)
+    for at in (0, 2 ** 31 - 50_000, dim - 5_000_000):
+        want = torch.round(x[0, at:at + 5_000_000].double() / float(s)).to(torch.int8)
+        assert torch.equal(codes[0, at:at + 5_000_000], want)
+    for at in range(0, dim, 1 << 28):  # the rest: every code within one of its value
+        off = (codes[0, at:at + (1 << 28)].float() * float(s) - x[0, at:at + (1 << 28)].float()).abs().max()
+        assert float(off) <= 0.5001 * float(s)
+
+
 @pytest.mark.parametrize("dtype", ("float16", "bfloat16"))
 def test_quantize_rows_of_few_bits(ctx, torch, dtype):
     """Half-precision values against every significand of the row's largest: quotients that are halves, or nearly so, are
