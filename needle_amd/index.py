@@ -71,6 +71,21 @@ def _value(t, what: str) -> int:
     return v
 
 
+_U32 = 2 ** 32 - 1
+
+
+def _check_u32(**sizes) -> None:
+    """Sizes that the library takes in 32 bits: ctypes would cut a longer number to its lowest 32."""
+    for name, value in sizes.items():
+        if value > _U32:
+            raise _lib.NeedleHipError(_lib.ERR_UNSUPPORTED, f"{name} = {value} does not fit 32 bits")
+
+
+def _check_end_token(end_token: int, vocab: int, rows: int, k: int) -> None:
+    if rows and k and not 0 <= end_token < vocab:  # (its lowest 32 bits could be)
+        raise _lib.NeedleHipError(_lib.ERR_INVALID_ARGUMENT, f"end_token {end_token} is not below vocab {vocab}")
+
+
 _torch_module = None
 
 
@@ -126,6 +141,7 @@ def _flat(t, name: str, dtype, size: int) -> None:
 
 def _codes_i8(codes, scales, what: str):
     """Host int8 codes [rows, dim] and their f32 scales, contiguous.  Values are not converted: a wider type would wrap."""
+    _check_u32(**{f"{name} of {what}": d for name, d in zip(("rows", "dim"), np.shape(codes))})
     c, s = np.ascontiguousarray(codes), _f32(scales).reshape(-1)
     if c.dtype != np.int8 or c.ndim != 2 or s.size != c.shape[0]:
         raise ValueError(f"{what} must be int8 [rows, dim] with one scale per row")
@@ -337,6 +353,8 @@ class Context:
         """(codes int8 [n, dim], scales f32 [n]) of float32 or float16 host rows: symmetric, scale = max |x| * (1 / 127) per row in f32,
         codes the whole numbers nearest to x / scale (needle_hip_quantize_rows_i8).  NaN / Inf raise InvalidVector."""
         r = np.asarray(rows)
+        if r.ndim == 2:
+            _check_u32(dim=r.shape[1])
         r = np.ascontiguousarray(r, dtype=np.float16 if r.dtype == np.float16 else np.float32)
         if r.ndim != 2:
             raise ValueError("rows must be [n, dim]")
@@ -349,6 +367,8 @@ class Context:
         """The same for a float32 / float16 / bfloat16 device matrix, into int8 [n, dim] codes and float32 [n] scales; rows may
         lie apart.  A row with a NaN or an infinity gets scale NaN and codes 0."""
         n, dim, apart = _rows_of(d_rows, "d_rows")
+        if dim > _U32:
+            _check_u32(dim=dim)
         value = _value(d_rows, "d_rows")
         _, _, codes_apart = _rows_of(d_codes, "d_codes", _I8, dim, n)
         _flat(d_scales, "d_scales", _F32, n)
@@ -383,6 +403,8 @@ class Context:
 
     def _product(self, d_a, d_a_scales, d_b, d_b_scales, d_out, d_bias) -> None:
         m, k, a_apart = _rows_of(d_a, "the rows", None if d_a_scales is None else _I8)
+        if (m | k) >> 32:
+            _check_u32(m=m, k=k)
         n, b_k, b_apart = _rows_of(d_b, "d_b", _I8)
         if b_k != k:
             raise _lib.DimensionMismatch(_lib.ERR_DIMENSION_MISMATCH, f"Dimension mismatch: {k} and {b_k}")
@@ -408,6 +430,7 @@ class Context:
         of `beams` rows of host logits [groups * beams, vocab], by total (normalize: scores + log-softmax; else scores +
         logits), then beam, then token (needle_hip_beam_select).  mask: bool [vocab] or [rows, vocab], True = admitted."""
         x = np.asarray(logits)
+        _check_u32(beams=beams, k=k, **dict(zip(("rows", "vocab"), x.shape)))
         x = np.ascontiguousarray(x, dtype=np.float16 if x.dtype == np.float16 else np.float32)
         if x.ndim != 2 or beams < 1 or x.shape[0] % beams:
             raise ValueError("logits must be [groups * beams, vocab]")
@@ -416,6 +439,8 @@ class Context:
         f = None if finished is None else np.ascontiguousarray(np.asarray(finished).reshape(-1) != 0, dtype=np.uint8)
         if (s is not None and s.size != rows) or (f is not None and f.size != rows):
             raise ValueError("scores and finished need one value per row of logits")
+        if f is not None:
+            _check_end_token(end_token, vocab, rows, k)
         words, stride = None, 0
         if mask is not None:
             b = np.asarray(mask, dtype=np.bool_)
@@ -443,6 +468,8 @@ class Context:
         `axis` (default 0) holds groups * beams rows in src and groups * k in dst; dst's rows become copies of their
         parents' (rows of unused places stay as they were)."""
         rows, vocab, apart = _rows_of(d_logits, "d_logits")
+        if (rows | vocab | beams | k) >> 32:
+            _check_u32(rows=rows, vocab=vocab, beams=beams, k=k)
         if beams < 1 or rows % beams:
             raise ValueError("d_logits must be [groups * beams, vocab]")
         groups, value = rows // beams, _value(d_logits, "d_logits")
@@ -450,6 +477,7 @@ class Context:
             _flat(d_scores, "d_scores", _F32, rows)
         if d_finished is not None:
             _flat(d_finished, "d_finished", _FLAGS, rows)
+            _check_end_token(end_token, vocab, rows, k)
         _flat(d_parents, "d_parents", _WORDS, groups * k)
         _flat(d_tokens, "d_tokens", _WORDS, groups * k)
         _flat(d_counts, "d_counts", _WORDS, groups)
@@ -474,6 +502,7 @@ class Context:
         if d_parents.dim() != 2 or beams < 1:
             raise ValueError("d_parents must be [groups, k]")
         groups, k = int(d_parents.shape[0]), int(d_parents.shape[1])
+        _check_u32(groups=groups, beams=beams, k=k)
         _flat(d_parents, "d_parents", _WORDS, groups * k)
         arr, n_states = self._states(states, groups, beams, k)
         self._check_device(d_parents)

@@ -159,6 +159,56 @@ def test_python_checks():
             call()
 
 
+def test_python_passes_no_size_that_32_bits_cut():
+    """Sizes and numbers the library takes in 32 bits are refused from 2^32 on, not cut to what is left of them: a row of 2^32 +
+    16 codes is not one of 16."""
+    import torch
+
+    from needle_amd import Context
+
+    c = Context.__new__(Context)
+    c.device, c._h = 0, C.c_void_p()
+    huge = (1 << 32) + 16
+
+    def on(*shape, dtype=torch.float32):
+        return torch.empty(*shape, dtype=dtype, device="meta")  # a shape, and no memory
+
+    def host(*shape, dtype=np.float32):
+        return np.broadcast_to(np.zeros((), dtype), shape)
+
+    i8, half = torch.int8, torch.float16
+    i, n = on(1, 2, dtype=torch.int32), on(1, dtype=torch.int32)
+
+    def sel(logits=on(1, 8), k=2, p=i, t=i, o=on(1, 2), cnt=n, beams=1, **kw):
+        return lambda: c.beam_select_device(logits, None, k, p, t, o, cnt, beams=beams, **kw)
+
+    wide = dict(p=on(1, huge, dtype=torch.int32), t=on(1, huge, dtype=torch.int32), o=on(1, huge))
+    many = dict(p=on(huge, 1, dtype=torch.int32), t=on(huge, 1, dtype=torch.int32), o=on(huge, 1), cnt=on(huge, dtype=torch.int32))
+    calls = [lambda: c.quantize_rows_device(on(1, huge, dtype=half), on(1, huge, dtype=i8), on(1)),
+             lambda: c.quantize_rows(host(1, huge)), lambda: c.quantize_rows(host(1, huge, dtype=np.float16)),
+             lambda: c.matmul_i8_device(on(1, huge, dtype=i8), on(1), on(2, huge, dtype=i8), on(2), on(1, 2)),
+             lambda: c.matmul_i8_device(on(huge, 3, dtype=i8), on(huge), on(1, 3, dtype=i8), on(1), on(huge, 1)),
+             lambda: c.linear_i8_device(on(1, huge), on(2, huge, dtype=i8), on(2), on(1, 2)),
+             lambda: c.linear_i8_device(on(huge, 3), on(1, 3, dtype=i8), on(1), on(huge, 1)),
+             lambda: c.matmul_i8(host(1, huge, dtype=np.int8), np.ones(1), host(2, huge, dtype=np.int8), np.ones(2)),
+             lambda: c.matmul_i8(host(huge, 3, dtype=np.int8), host(huge), host(2, 3, dtype=np.int8), np.ones(2)),
+             sel(logits=on(1, huge)), sel(k=huge, **wide), sel(logits=on(huge, 1), k=1, **many), sel(logits=on(0, 8), beams=huge, k=1, p=i[:0], t=i[:0], o=on(0, 1), cnt=n[:0]),
+             lambda: c.beam_select(host(1, huge), None, 2, beams=1), lambda: c.beam_select(host(huge, 1), None, 2, beams=1),
+             lambda: c.beam_select(host(1, 8), None, huge, beams=1),
+             lambda: c.beam_reorder_device(on(1, 2, dtype=torch.int32), [(on(huge, 1, dtype=i8), on(2, 1, dtype=i8))], beams=huge),
+             lambda: c.beam_reorder_device(on(1, huge, dtype=torch.int32), [(on(2, 1, dtype=i8), on(huge, 1, dtype=i8))], beams=2),
+             lambda: c.beam_reorder_device(on(huge, 1, dtype=torch.int32), [(on(huge, 1, dtype=i8), on(huge, 1, dtype=i8))], beams=1)]
+    for j, call in enumerate(calls):
+        with pytest.raises(_lib.NeedleHipError) as e:
+            call()
+        assert e.value.status == UNSUPPORTED and str(huge) in str(e.value), j
+    for end in (-1, huge, (1 << 32) + 3):  # an end token that is one of the vocabulary only in its lower 32 bits
+        for call in (sel(d_finished=on(1, dtype=torch.bool), end_token=end), lambda: c.beam_select(np.zeros((1, 8)), None, 2, beams=1, finished=[0], end_token=end)):
+            with pytest.raises(_lib.NeedleHipError) as e:
+                call()
+            assert e.value.status == ARG and str(end) in str(e.value)
+
+
 def test_structs_and_constants_mirror_the_header():
     import os
     import re
