@@ -539,7 +539,9 @@ needle_hip_status needle_hip_quantize_rows_i8_device(needle_hip_ctx* ctx, const 
  * output channels of a layer).  The sum is exact in 32-bit integers, which k <= 131071
  * guarantees for any codes (-128 included); it is turned into f32, multiplied by the
  * two scales in that order, the bias (nullable) is added, and the result is rounded once
- * more where out_value (needle_value) is a half type.  k may be a prefix of longer rows (stride
+ * more where out_value (needle_value) is a half type.  Large products of rows that do not all
+ * start on 16 bytes copy them into the context's workspace where there is room (2.4 GB at most,
+ * kept until the context closes).  k may be a prefix of longer rows (stride
  * above k).  m, n < 2^31; m * n may be any size.  k 0 gives the bias, or zeros. */
 needle_hip_status needle_hip_matmul_i8(needle_hip_ctx* ctx, const int8_t* a, const float* a_scales, uint32_t m,
                                        const int8_t* b, const float* b_scales, uint64_t n, uint32_t k,

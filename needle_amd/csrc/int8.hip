@@ -724,9 +724,17 @@ static hipError_t launch_slab(needle_hip_ctx* c, MatmulParams p, int out_value) 
     // 513 62, 64; not so 300 x 66000 x 513 63, 46; 2000 x 2000 x 301 11, 7.
     const uint32_t stride = (p.k + 63) / 64 * 64;
     const uint64_t bytes = (p.n + p.m) * stride;
-    if (!rows_aligned(p) && tiles_of(p, 128, 128) > (uint64_t)c->n_cu && p.m * p.n >= 512 * (p.m + p.n) && bytes <= ALIGN_MOST) {
+    bool copy = !rows_aligned(p) && tiles_of(p, 128, 128) > (uint64_t)c->n_cu && p.m * p.n >= 512 * (p.m + p.n) && bytes <= ALIGN_MOST;
+    if (copy) {
         const hipError_t e = c->scratch[5].ensure(bytes);
-        if (e != hipSuccess) return e;
+        if (e == hipErrorOutOfMemory) {  // the product needs no copies: on as the rows are
+            (void)hipGetLastError();
+            copy = false;
+        } else if (e != hipSuccess) {
+            return e;
+        }
+    }
+    if (copy) {
         int8_t* to = c->scratch[5].as<int8_t>();
         hipLaunchKernelGGL(align_rows_kernel, dim3((uint32_t)((p.n + p.m + 3) / 4)), dim3(256), 0, c->stream, p, to, stride);
         p.b = to;

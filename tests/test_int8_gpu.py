@@ -292,6 +292,38 @@ def test_matmul_behind_four_billion(ctx, torch):
     _check_product(out, x, sa[:3], x, sb[:3], None, "float32")
 
 
+def test_a_product_without_room_for_its_copies(torch):
+    """Rows that the loads cannot take as they are get copied to aligned ones where that is faster; on a device without room
+    for the copies the product is made without them."""
+    import needle_amd as na
+
+    m, n, k = 7000, 12_000, 100_001  # copies of 1.9e9 bytes
+    g = torch.Generator(device="cuda").manual_seed(11)
+    a, sa = _table(torch, g, m, k)
+    b, sb = _table(torch, g, n, k)
+    out = torch.full((m, n), float("nan"), device="cuda")
+    c = na.Context(0)
+    try:
+        c.matmul_i8_device(a[:40, :64], sa[:40], b[:40, :64], sb[:40], torch.empty(40, 40, device="cuda"))
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        left = torch.cuda.mem_get_info()[0] - (1 << 30)
+        full = torch.empty(left, dtype=torch.uint8, device="cuda")
+        assert torch.cuda.mem_get_info()[0] < (m + n) * k
+        c.matmul_i8_device(a, sa, b, sb, out)
+        del full
+        torch.cuda.empty_cache()
+        again = torch.full((m, n), float("nan"), device="cuda")
+        c.matmul_i8_device(a, sa, b, sb, again)  # with room
+    finally:
+        c.close()
+    assert torch.equal(out, again)
+    at, bt = (torch.randint(0, r, (300,), generator=g, device="cuda") for r in (m, n))
+    acc = torch.stack([(a[i].double() * b[j].double()).sum() for i, j in zip(at.tolist(), bt.tolist())])
+    exact = acc * sa[at].double() * sb[bt].double()
+    assert ((out[at, bt].double() - exact).abs() <= 3.01 * HALF_STEP["float32"] * exact.abs()).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 40, 33), (4, 1000, 1024), (37, 130, 301), (300, 520, 768), (2, 3, 0), (1, 8192, 8192), (16, 300, 511), (5, 17_000, 300),
                                    (13, 33_000, 630), (3, 1, 2047), (16, 70_000, 400), (2, 4099, 4096)])
