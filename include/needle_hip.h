@@ -591,8 +591,9 @@ typedef struct needle_beam_params {
 /* Something every beam carries (keys and values, a query vector, a history): after the
  * picks, row g * k + j of dst becomes a copy of row g * beams + parent of src.  A row is
  * outer x inner runs of `bytes` bytes; all strides are in bytes.  Rows of places without
- * a pick stay as they were.  dst must not overlap any src, another dst or another array
- * of the call. */
+ * a pick stay as they were.  dst must share no byte with any src, another dst or another
+ * array of the call; states may lie between each other's runs (keys and values as parts of
+ * one array's rows) where one of their strides is a period of both. */
 typedef struct needle_beam_state {
     const void* src;
     void* dst;

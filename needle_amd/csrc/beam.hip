@@ -703,18 +703,52 @@ static void launch_join(const BeamParams& p, bool normalize, hipStream_t stream)
 }
 
 struct ByteRange { const void* p; uint64_t n; };
+// Runs of `bytes` bytes from `base` on along three axes; `span` bytes from the first to behind the last.
+struct Axis { uint64_t n, stride; };
+struct Runs {
+    uint64_t base, bytes, span;
+    Axis ax[3];
+    // one period of them, `at` bytes from its start: without the axes that step by whole periods
+    Runs within(uint64_t period, uint64_t at) const {
+        Runs r{at, bytes, bytes, {}};
+        for (int i = 0; i < 3; ++i)
+            if (ax[i].n > 1 && ax[i].stride % period) {
+                r.ax[i] = ax[i];
+                r.span += (ax[i].n - 1) * ax[i].stride;
+            }
+        return r;
+    }
+};
+// Two arrays of runs share no byte: one lies behind the other, or they share none of a period that one of their strides
+// makes and that neither's runs leave (parts of the rows, the layers or the runs of one array).  Every period leaves out
+// an axis, so this ends.
+static bool share_nothing(const Runs& a, const Runs& b) {
+    if (!a.span || !b.span || a.base + a.span <= b.base || b.base + b.span <= a.base) return true;
+    for (const Runs* r : {&a, &b})
+        for (const Axis& x : r->ax) {
+            if (x.n <= 1 || !x.stride) continue;
+            const uint64_t far = a.base < b.base ? (b.base - a.base) % x.stride : (a.base - b.base) % x.stride;
+            for (const uint64_t at : {far, (x.stride - far) % x.stride}) {  // (the first run of either may start the period)
+                const bool later = (a.base < b.base) == (at == far);  // b's does not
+                const Runs first = (later ? a : b).within(x.stride, 0), second = (later ? b : a).within(x.stride, at);
+                if (first.span <= x.stride && second.span <= x.stride - at && share_nothing(first, second)) return true;
+            }
+        }
+    return false;
+}
 // `others`: arrays of the same call that no dst may overlap
 static needle_hip_status states_check(const needle_beam_state* states, uint32_t n_states, uint64_t rows, uint64_t picks, const ByteRange* others,
                                       int n_others) {
     if (n_states && !states) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "states is null");
     if (n_states > STATES_MAX) return fail(NEEDLE_HIP_ERR_UNSUPPORTED, "at most %u states per call", STATES_MAX);
-    struct Range { uint64_t first, second; } from[STATES_MAX] = {}, to[STATES_MAX] = {};  // first byte, last byte + 1
+    Runs from[STATES_MAX], to[STATES_MAX];  // set as far as there are states
     for (uint32_t i = 0; i < n_states; ++i) {
         const needle_beam_state& s = states[i];
+        from[i].span = to[i].span = 0;
         if (s.outer == 0 || s.inner == 0 || s.bytes == 0) continue;
         if (!s.src || !s.dst) return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "state %u has a null pointer", i);
         // rows, outer and inner runs of dst lie apart in one of their orders: no byte is written twice
-        struct Axis { uint64_t n, stride; } ax[3] = {{s.outer, s.dst_outer_stride}, {picks, s.dst_row_stride}, {s.inner, s.dst_inner_stride}};
+        Axis ax[3] = {{s.outer, s.dst_outer_stride}, {picks, s.dst_row_stride}, {s.inner, s.dst_inner_stride}};
         std::sort(ax, ax + 3, [](const Axis& a, const Axis& b) { return a.n > 1 && b.n > 1 ? a.stride < b.stride : a.n > b.n; });
         uint64_t span = s.bytes, last;
         for (const Axis& a : ax) {
@@ -728,17 +762,17 @@ static needle_hip_status states_check(const needle_beam_state* states, uint32_t 
         for (const Axis& a : sx)
             if (a.n == 0 || __builtin_mul_overflow(a.n - 1, a.stride, &last) || __builtin_add_overflow(reach, last, &reach) || reach > (1ull << 62))
                 return fail(NEEDLE_HIP_ERR_UNSUPPORTED, "state %u spans more than 2^62 bytes", i);
-        from[i] = {(uint64_t)s.src, (uint64_t)s.src + reach};
-        to[i] = {(uint64_t)s.dst, (uint64_t)s.dst + span};
+        from[i] = {(uint64_t)s.src, s.bytes, reach, {sx[0], sx[1], sx[2]}};
+        to[i] = {(uint64_t)s.dst, s.bytes, span, {ax[0], ax[1], ax[2]}};
         for (int o = 0; o < n_others; ++o)
             if (ranges_meet(s.dst, span, others[o].p, others[o].n))
                 return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "dst of state %u overlaps another array of the call", i);
     }
     for (uint32_t i = 0; i < n_states; ++i)
         for (uint32_t j = 0; j < n_states; ++j) {
-            if (to[i].first < from[j].second && from[j].first < to[i].second)
+            if (!share_nothing(to[i], from[j]))
                 return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "dst of state %u overlaps src of state %u", i, j);
-            if (i != j && to[i].first < to[j].second && to[j].first < to[i].second)
+            if (i < j && !share_nothing(to[i], to[j]))
                 return fail(NEEDLE_HIP_ERR_INVALID_ARGUMENT, "dst of state %u overlaps dst of state %u", i, j);
         }
     return NEEDLE_HIP_OK;

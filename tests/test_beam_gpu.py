@@ -336,6 +336,26 @@ def test_reorder_alone(ctx, torch):
     ctx.beam_reorder_device(parents[:0], [(src[:0], dst[:0])], beams=3)
 
 
+def test_states_that_interleave_in_one_array(ctx, torch):
+    """Keys and values of several layers, a beam's all in one row, and as pairs of runs."""
+    groups, beams, k = 3, 4, 5
+    g = torch.Generator(device="cuda").manual_seed(14)
+    src = torch.randn(groups * beams, 2, 3, 7, 64, generator=g, device="cuda")  # rows, keys / values, layers, heads, dims
+    dst = torch.randn(groups * k, 2, 3, 7, 64, generator=g, device="cuda")
+    parents = torch.randint(0, beams, (groups, k), generator=g, device="cuda", dtype=torch.int32)
+    parents[1, 2] = -1
+    want = _moved(torch, src, dst, parents.cpu(), beams)
+    for parts in ([lambda t, j=j: t[:, j] for j in range(2)], [lambda t, j=j, y=y: t[:, j, y] for j in range(2) for y in range(3)],
+                  [lambda t, j=j: t[:, :, :, j] for j in range(7)], [lambda t, j=j: t.reshape(t.shape[0], 42, 2, 32)[:, :, j] for j in range(2)]):
+        out = dst.clone()
+        ctx.beam_reorder_device(parents, [(part(src), part(out)) for part in parts], beams=beams)
+        assert torch.equal(out, want)
+    out = dst.clone()
+    with pytest.raises(Exception, match="overlaps"):
+        ctx.beam_reorder_device(parents, [(src[:, 0], out[:, 0]), (src[:, :, 0], out[:, :, 0])], beams=beams)
+    assert torch.equal(out, dst)
+
+
 def test_states_behind_four_gigabytes(ctx, torch):
     rows = torch.randint(-128, 128, (4, 2 ** 31 - 77), device="cuda", dtype=torch.int8)  # offsets of rows 2 and 3 pass 2^32
     dst = torch.zeros(4, 2 ** 31 - 77, device="cuda", dtype=torch.int8)

@@ -108,6 +108,58 @@ def test_states(states, status):
         assert select(states=(_lib.BeamState * 1)(_lib.BeamState(**state())), n_states=1, **other) == ARG
 
 
+def _bytes_of(s, side, rows):
+    outer, row, inner = (s[f"{side}_{axis}_stride"] for axis in ("outer", "row", "inner"))
+    return {s[side] + o * outer + r * row + i * inner + b for o in range(s["outer"]) for r in range(rows) for i in range(s["inner"]) for b in range(s["bytes"])}
+
+
+def test_states_that_share_an_array_and_no_byte():
+    """Keys and values as parts of every row, of every layer or of every run of one array lie between each other; a byte
+    more and they overlap."""
+    nothing_to_refuse = (_lib.ERR_HIP, OK)  # (only the device is missing)
+
+    def pair(first, second):
+        out = []
+        for off in (first, second):
+            out.append(dict(state(), src=at(1 << 16) + off, dst=at(1 << 17) + off))
+        return out
+
+    rows = dict(src_row_stride=160, dst_row_stride=160)  # six rows of two parts of 72 bytes (two runs of 32, 40 apart)
+    apart = [[dict(s, **rows) for s in pair(0, 80)], [dict(s, **rows) for s in pair(88, 0)], [dict(s, **rows, outer=2, src_outer_stride=6 * 160, dst_outer_stride=8 * 160) for s in pair(0, 80)],
+             pair(0, 0)[:1] + [dict(pair(0, 0)[1], src=at(1 << 16) + 32, dst=at(1 << 17) + 32, bytes=8)],  # in the gaps of the runs
+             [dict(s, **rows, inner=4, bytes=20, src_inner_stride=40, dst_inner_stride=40) for s in pair(0, 20)]]
+    for states in apart:
+        assert reorder(*states) in nothing_to_refuse and reorder(*states[::-1]) in nothing_to_refuse
+    meet = [[dict(s, **rows) for s in pair(0, 71)], [dict(s, **rows) for s in pair(0, 89)], [dict(s, **rows) for s in pair(0, 0)],
+            pair(0, 0)[:1] + [dict(pair(0, 0)[1], src=at(1 << 16) + 32, dst=at(1 << 17) + 32, bytes=9)],
+            [dict(s, **rows, inner=4, bytes=21, src_inner_stride=40, dst_inner_stride=40) for s in pair(0, 20)]]
+    for states in meet:
+        assert reorder(*states) == ARG and reorder(*states[::-1]) == ARG
+    # a dst between the rows of a src
+    assert reorder(state(dst=at((1 << 16) + 80), src_row_stride=160, dst_row_stride=160)) in nothing_to_refuse
+    assert reorder(state(dst=at((1 << 16) + 71), src_row_stride=160, dst_row_stride=160)) == ARG
+    rng = np.random.default_rng(0)
+    taken = 0
+    for _ in range(3000):  # whatever shares a byte is refused, whatever the strides
+        stride = [int(v) for v in rng.choice([8, 12, 24, 48, 50, 96, 100, 200, 400], 6)]
+        both = []
+        for j in range(2):
+            o, r, i = stride[:3] if rng.random() < 0.6 else stride[3:]
+            both.append(dict(src=at(1 << 18) + j * (1 << 15), dst=at(1 << 17) + int(rng.integers(0, 120)), outer=int(rng.integers(1, 3)), inner=int(rng.integers(1, 4)),
+                             bytes=int(rng.integers(1, 25)), src_outer_stride=8192, src_row_stride=1024, src_inner_stride=64, dst_outer_stride=o,
+                             dst_row_stride=r, dst_inner_stride=i))
+        if any(reorder(s) == ARG for s in both):  # (its own rows overlap)
+            continue
+        one, two = (_bytes_of(s, "dst", 8) for s in both)
+        got = reorder(*both)
+        if one & two:
+            assert got == ARG, both
+        elif max(one) < min(two) or max(two) < min(one):
+            assert got in nothing_to_refuse, both
+        taken += got in nothing_to_refuse
+    assert taken > 20
+
+
 def test_state_layouts():
     import torch
 
