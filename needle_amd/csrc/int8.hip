@@ -748,13 +748,21 @@ static hipError_t launch_slab(needle_hip_ctx* c, MatmulParams p, int out_value) 
     }
 }
 
-// Slabs of rows whose grids stay below 2^32 threads.
-constexpr uint64_t SLAB_N = 1ull << 26, SLAB_M = 1ull << 22;
+// Slabs of rows whose grids stay below 2^32 threads, the most a launch takes: the largest have a workgroup of 512 for every
+// tile of 128 x 128 (smaller tiles are taken for products of few).
+constexpr uint64_t SLAB_N = 1ull << 26, SLAB_M = 1ull << 22, SLAB_TILES = 1ull << 22;
+constexpr uint64_t slab_rows(uint64_t n) {  // of a, against n <= SLAB_N rows of b
+    const uint64_t rows = SLAB_TILES / ((n + 127) / 128) * 128;
+    return rows < SLAB_M ? rows : SLAB_M;
+}
+static_assert(slab_rows(SLAB_N) >= 128 && (slab_rows(SLAB_N) / 128) * (SLAB_N / 128) * 512 < (1ull << 32) &&
+              (slab_rows((1u << 22) + 1) / 128) * ((1u << 15) + 1) * 512 < (1ull << 32), "a launch takes the grid");
 static hipError_t launch_matmul_i8(needle_hip_ctx* c, const MatmulParams& p, int out_value) {
-    for (uint64_t i = 0; i < p.m; i += SLAB_M)
+    const uint64_t most = slab_rows(std::min(SLAB_N, p.n));
+    for (uint64_t i = 0; i < p.m; i += most)
         for (uint64_t j = 0; j < p.n; j += SLAB_N) {
             MatmulParams q = p;
-            q.m = (uint32_t)std::min(SLAB_M, p.m - i);
+            q.m = (uint32_t)std::min(most, p.m - i);
             q.n = std::min(SLAB_N, p.n - j);
             q.a += i * p.a_stride;
             q.a_scales += i;

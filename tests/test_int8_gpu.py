@@ -292,6 +292,28 @@ def test_matmul_behind_four_billion(ctx, torch):
     _check_product(out, x, sa[:3], x, sb[:3], None, "float32")
 
 
+def test_a_product_of_eight_million_tiles(ctx, torch):
+    """An output of 275 GB, of as many 128 x 128 tiles as one launch has no grid for."""
+    m, n, k = 2050, 1 << 26, 16
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < m * n * 2 + (4 << 30):
+        pytest.skip("the output does not fit this device")
+    g = torch.Generator(device="cuda").manual_seed(13)
+    a, sa = _table(torch, g, m, k)
+    b, sb = _table(torch, g, n, k)
+    out = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    rows, cols = (slice(0, 70), slice(980, 1100), slice(1990, 2050)), (slice(0, 300), slice(2 ** 25 - 100, 2 ** 25 + 100), slice(n - 300, n))
+    for r in rows:
+        for c in cols:
+            out[r, c] = float("nan")
+    ctx.matmul_i8_device(a, sa, b, sb, out)
+    for r in rows:
+        for c in cols:
+            _check_product(out[r, c], a[r], sa[r], b[c], sb[c], None, "bfloat16")
+    del out
+    torch.cuda.empty_cache()
+
+
 def test_a_product_without_room_for_its_copies(torch):
     """Rows that the loads cannot take as they are get copied to aligned ones where that is faster; on a device without room
     for the copies the product is made without them."""
