@@ -46,7 +46,7 @@ __device__ inline double exp64(double x) {
 // The same with the 128 powers 2^(j / 128) in LDS, for one exponential per logit: n counts 128ths, and what is left is so
 // small that g takes four nodes (1.5e-16); with the roundings e^x is 4 + |x| units of 2^-53 off at most.  A power lies there
 // less its number j in the exponent's lowest bits, so that adding n there gives 2^(n / 128).  Twelve f64 instructions per
-// logit, its place in the sum among them; without powers it would be eighteen (64 x 8 rows of 131072 bf16 logits: 8 us more).
+// logit, its place in the sum among them; without powers it would be eighteen (64 x 8 rows of 131072 bf16 logits: 77 us instead of 66).
 constexpr int POWER_BITS = 7, POWERS = 1 << POWER_BITS;
 __device__ inline void fill_powers(double* powers, int t) {
     if (t >= POWERS) return;
@@ -157,6 +157,7 @@ struct BeamParams {
 // places and values of its row alone: equal rows have equal sums.
 //
 // Not normalized it is bound by the bytes: 32 x 10 x 100003 f32, k = 64, take 30 us (4.3 TB/s).
+// Normalized the f64 instructions bound it: 64 x 8 x 131072, k = 8, take 66 us in bf16, 74 in f32 (3.6 TB/s).
 template <typename V, int EACH, int GROUPS, bool NORMALIZE, bool MASKED>
 __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p) {
     constexpr int WIDE = 16 / V::size, LOADS = EACH / WIDE, CAP = 1024, MINE = CAP / PIECE_THREADS;
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(PIECE_THREADS) void beam_piece_kernel(BeamParams p)
     for (int g = 0; g < GROUPS; ++g) run[g] = -__builtin_inff();
     // The thread's sum of exponentials, in units of exp(ref): ref is the largest logit of the workgroup when the bound was last
     // raised, or a larger one of this thread since.  (In units of the thread's own largest, which grows in most of the first
-    // chunks, 64 x 8 rows of 131072 logits take 2.5 us longer in f32, 0.5 in bf16.)
+    // chunks, 64 x 8 rows of 131072 logits take 77 us instead of 74 in f32, 67.5 instead of 66.4 in bf16.)
     double sum = 0.0;
     float ref = -__builtin_inff(), highest = ref;
     bool nan = false;
@@ -666,11 +667,11 @@ static hipError_t launch_moves(const uint32_t* d_parents, uint32_t groups, uint3
 }
 
 // ---- host side ---------------------------------------------------------------------------------
-// Bytes of a row per thread and chunk: 64 x 8 rows of 131072 bf16 logits take a third longer with 64, whose registers leave
-// room for three workgroups per CU.
+// Bytes of a row per thread and chunk.  Us with 32 and with 64: 64 x 8 rows of 131072 logits in bf16 66 and 65, in f32 74 and
+// 70; 10 rows of 131000 in bf16, k = 64, 14.2 and 15.0; 4 rows of 32000 in f32 5.8 and 7.3.
 constexpr uint32_t CHUNK_BYTES = 32;
-// Workgroups per CU that the pieces are cut for: the same rows take 70 us
-// with 4, 76 with 5, 73 with 8; 32 x 10 rows of 100003 f32 logits, not normalized, 30, 30 and 33.
+// Workgroups per CU that the pieces are cut for: the bf16 rows of 131072 take 66 us with 4, 72 with 5, 69 with 8; 32 x 10 rows of
+// 100003 f32 logits, not normalized, 30, 30 and 33.
 constexpr uint32_t PIECES_PER_CU = 4;
 // What a chunk takes a piece: 1 to 3 us, more with the logarithm and with a larger k.  10 rows of 131000 bf16 logits, k = 64,
 // take 23 us with pieces cut for it and 34 with a piece per chunk; 4 rows of 1500000 34, and 42 where it is a tenth.

@@ -32,7 +32,7 @@ constexpr float TINY_ROW = 0x1p-60f, TINY_UP = 0x1p80f;
 // LANES lanes (256: the four waves of a workgroup) hold a row in registers, PER vectors of WIDE values each, so that it is
 // read once: 16 bytes per lane and load, from any address, WIDE codes per store.  Rows longer than 256 * 8 * WIDE values are
 // read twice (the second time from the cache) by a workgroup of 1024.  The bytes bound it: 200003 x 384 f32 take 68 us, 5.6
-// TB/s (a wave per row, a value per load, read twice: 174 us); 41593 x 1505 bf16 35 us, 5.4 TB/s (with every residue taken, a
+// TB/s (a wave per row, a value per load, read twice: 174 us); 41593 x 1505 bf16 37 us, 5.1 TB/s (with every residue taken, a
 // dozen instructions more per value, 54).
 //
 // Of a row that is neither tiny nor NaN most codes need no residue: x / s and x * (1 / s) differ by 127 * 2^-24 at most, so
