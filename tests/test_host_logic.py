@@ -159,3 +159,16 @@ def test_transparent_fallback_manager():  # gpu/mod.rs:1407-1560; tests :2228-22
         with pytest.raises(na._lib.NeedleHipError):
             strict.search(query, vectors, 1, na.DistanceType.Cosine)
     assert strict.gpu_failures == 4  # the fifth call found the device path switched off
+
+
+def test_streams_have_the_default_priority():
+    """Work on streams of different priorities that wait for one another's events has hung: no source asks for a priority."""
+    import glob
+    import os
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    sources = [f for pattern in ("needle_amd/csrc/*.hip", "needle_amd/csrc/*.h", "needle_amd/*.py", "bench.py", "tools/*.py") for f in glob.glob(os.path.join(root, pattern))]
+    assert len(sources) > 20
+    for f in sources:
+        text = open(f).read()
+        assert "StreamCreateWithPriority" not in text and "Stream(priority" not in text and "is_high_priority_stream" not in text, f
